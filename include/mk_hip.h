@@ -50,6 +50,10 @@ extern "C" {
 #define MK_MODE_F32 0
 #define MK_MODE_Q8 1
 
+/* Element type of the rows that the token-mixer calls take and return (head norm + rotation, 4-bit KV cache, linear attention). */
+#define MK_F32 0
+#define MK_BF16 1
+
 /* Activation rule of a packed expert (see mk_dev_moe_decode). */
 #define MK_ACT_SWIGLU 0 /* silu(g) * u, silu(x) = x / (1 + exp(-x))            (src/deepseek.rs:1086) */
 #define MK_ACT_SITU 1   /* 4 tanh(g/4) sigmoid(g) * 25 tanh(u/25)                (src/model.rs:619-621)  */
@@ -410,6 +414,80 @@ size_t mk_mla_heads_workspace_bytes(size_t m, size_t nh, size_t nope, size_t vd)
 int mk_dev_mla_heads_q8_attn(const int8_t *kq, const float *ks, const float *kr, const int8_t *vq, const float *vs, size_t pos0,
                              const float *q, size_t m, size_t nh, size_t nope, size_t rope, size_t vd, float scale, int hadamard,
                              void *workspace, float *out, void *stream);
+
+/* ------------------------------------------- device level: token mixers */
+
+/* These calls have no counterpart in the reference's hot path; rows are f32 or bfloat16 (dtype: MK_F32, MK_BF16), sums, norms,
+ * softmax statistics and states f32, and a bfloat16 result is rounded once.
+ *
+ * A batch of sequences: the rows of a call lie one behind the other, cu [B + 1] int32 (device) says where each sequence's
+ * begin and the last one's end; cu NULL: T / B rows each (T % B == 0).  Entries of cu outside 0 .. T are taken as the nearer
+ * bound; rows that belong to no sequence are neither read nor written.  A token's heads are contiguous, tokens may be
+ * further apart (a row stride in values, a multiple of 8: q, k, v may be slices of one projection's rows).
+ *
+ * mk_dev_qk_norm_rope: RMS norm of every query head [T][nh][hd] and key head [T][nkv][hd] with the rotation of the token's
+ * position, one pass:
+ *   r = x / sqrt(mean(x^2) + eps) * w       norm != 0; wq, wk [hd] f32 or NULL (ones); norm == 0: r = x * w
+ *   (a, b) -> (a c - b s, a s + b c)        on the rot values from rot_at on, (a, b) = (2 i, 2 i + 1), or, halves != 0,
+ *                                           (i, i + rot / 2); c, s = cos, sin [n_pos][rot / 2] f32 at row pos[t], entry i
+ * pos [T] int32 (may be NULL when rot == 0).  A token whose position is negative is padding: its rows of q_out and k_out stay
+ * as they are; at a position of n_pos or more the rotated values become NaN.  nh or nkv may be 0.  In place is allowed
+ * (q_out == q with the same stride).  hd a multiple of 8 up to 512, rot of 16, rot_at of 8; pointers 16-byte aligned. */
+int mk_dev_qk_norm_rope(int dtype, const void *q, size_t q_stride, size_t nh, const void *k, size_t k_stride, size_t nkv, size_t T,
+                        size_t hd, int norm, const float *wq, const float *wk, float eps, const float *cos, const float *sin, size_t n_pos,
+                        const int32_t *pos, size_t rot, size_t rot_at, int halves, void *q_out, size_t q_out_stride, void *k_out,
+                        size_t k_out_stride, void *stream);
+
+/* A KV cache held in 4 bits, for B sequences of up to cap positions: per kv head K rows of dk and V rows of dv values as MXFP4 (low
+ * nibble = even value, an e8m0 byte per 32), and, rope != 0, a tail of `rope` K values that the heads share, as bfloat16 (a
+ * rotated part is small and sensitive: 2 bytes a value of a row that all heads share).  All device memory:
+ *   kq [B][nkv][cap][dk/2]  ks [B][nkv][cap][dk/32]  kr [B][cap][rope]  vq [B][nkv][cap][dv/2]  vs [B][nkv][cap][dv/32]
+ *   lens [B] int32: the positions each sequence holds
+ * dk, dv multiples of 32 up to 512, rope a multiple of 8 up to 64; arrays 16-byte aligned.
+ * A block's exponent is the smallest e with 6 * 2^e >= max|x| within [-127, 125], a value's level the nearest (upwards at a
+ * midpoint).  NaN is held as 0, infinities and what lies beyond 6 * 2^125 as the largest level: what is read back is finite
+ * (the bfloat16 tail keeps NaN and infinities). */
+typedef struct {
+    size_t B, nkv, dk, rope, dv, cap;
+    uint8_t *kq, *ks, *vq, *vs;
+    uint16_t *kr;
+    int32_t *lens;
+} mk_kv4_cache;
+
+/* Row i of a sequence's rows in this call goes to its position lens + i, then lens grows by their number (fresh != 0: the
+ * sequences are emptied first).  k_rows [T][nkv][dk + rope] (the tail is taken from head 0), v_rows [T][nkv][dv].  A row at a
+ * position of cap or more is not stored; lens counts it all the same (see mk_dev_kv4_attn). */
+int mk_dev_kv4_append(const mk_kv4_cache *c, int dtype, const void *k_rows, size_t k_stride, const void *v_rows, size_t v_stride, size_t T,
+                      const int32_t *cu, int fresh, void *stream);
+
+/* The values of the first n positions: k [B][n][nkv][dk + rope], v [B][n][nkv][dv]; zeros where a sequence holds none. */
+int mk_dev_kv4_to_f32(const mk_kv4_cache *c, size_t n, float *k, float *v, void *stream);
+
+/* Softmax attention of the rows that were appended last: with m rows of a sequence in this call, row i attends its positions
+ * 0 ..= lens - m + i (m = 1: a decode step; more: a prompt, causal).  q [T][nh][dk + rope], out [T][nh][dv] contiguous; query
+ * head h reads kv head h / (nh / nkv).  s_j = scale * q . k_j, out = sum softmax(s)_j v_j.  A row that has no position to
+ * attend (an empty sequence) gives zeros, one that would have to attend a position beyond cap gives NaN.
+ * max_len: an upper bound of lens, if the caller has one (0: none); it only steers how the work is split.
+ * workspace: mk_kv4_attn_workspace_bytes(c, T, nh) bytes, 256-byte aligned, one for each call that may run at the same time. */
+size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh);
+int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_stride, size_t T, const int32_t *cu, size_t nh, float scale,
+                    size_t max_len, void *workspace, void *out, void *stream);
+
+/* Linear attention with a decay for each head:
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,  o_t = scale * S_t^T q_t        per value head; S [dk][dv] f32
+ * q, k [T][nkh][dk], v [T][nh][dv], out [T][nh][dv] contiguous (value head h reads key head h / (nh / nkh)); g: log decays f32,
+ * [T] rows of nh at g_stride, or, g_stride == 0, one constant per head [nh]; -inf empties the state.  state [B][nh][dk][dv]
+ * (NULL: zeros) is the state before the call, state_out the one after it; they may be the same memory.  A sequence without
+ * tokens keeps its state.  dk, dv multiples of 8 up to 256; pointers 16-byte aligned.
+ * _attn is the form for prompts (workspace: mk_linear_attn_workspace_bytes, 256-byte aligned, one for each call that may run
+ * at the same time), _step the one for a single token of each of B sequences (rows b of q, k, v, g and out). */
+size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv);
+int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
+                       size_t g_stride, size_t T, const int32_t *cu, size_t B, size_t nh, size_t nkh, size_t dk, size_t dv, float scale,
+                       const float *state, float *state_out, void *workspace, void *out, void *stream);
+int mk_dev_linear_attn_step(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride,
+                            const float *g, size_t g_stride, size_t B, size_t nh, size_t nkh, size_t dk, size_t dv, float scale,
+                            const float *state, float *state_out, void *out, void *stream);
 
 /* ---------------------------------- device level: prefill expert GEMM */
 

@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libmk_hip.so")
 MK_OK = 0
 MODE_F32, MODE_Q8 = 0, 1
 ACT_SWIGLU, ACT_SITU, ACT_DS = 0, 1, 2
+F32, BF16 = 0, 1
 
 
 class MkError(RuntimeError):
@@ -38,6 +39,11 @@ class Prof(C.Structure):
 
 class PrefillLayout(C.Structure):
     _fields_ = [("order", C.c_size_t), ("pos", C.c_size_t), ("offsets", C.c_size_t), ("g", C.c_size_t), ("u", C.c_size_t), ("o", C.c_size_t)]
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("B", C.c_size_t), ("nkv", C.c_size_t), ("dk", C.c_size_t), ("rope", C.c_size_t), ("dv", C.c_size_t), ("cap", C.c_size_t),
+                ("kq", C.c_void_p), ("ks", C.c_void_p), ("vq", C.c_void_p), ("vs", C.c_void_p), ("kr", C.c_void_p), ("lens", C.c_void_p)]
 
 
 def _load():
@@ -106,6 +112,14 @@ def _load():
         "mk_dev_mla_heads_to_f32": (i32, [vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, i32, vp, vp, vp]),
         "mk_mla_heads_workspace_bytes": (sz, [sz, sz, sz, sz]),
         "mk_dev_mla_heads_q8_attn": (i32, [vp, vp, vp, vp, vp, sz, vp, sz, sz, sz, sz, sz, f32, i32, vp, vp, vp]),
+        "mk_dev_qk_norm_rope": (i32, [i32, vp, sz, sz, vp, sz, sz, sz, sz, i32, vp, vp, f32, vp, vp, sz, vp, sz, sz, i32, vp, sz, vp, sz, vp]),
+        "mk_dev_kv4_append": (i32, [C.POINTER(Kv4Cache), i32, vp, sz, vp, sz, sz, vp, i32, vp]),
+        "mk_dev_kv4_to_f32": (i32, [C.POINTER(Kv4Cache), sz, vp, vp, vp]),
+        "mk_kv4_attn_workspace_bytes": (sz, [C.POINTER(Kv4Cache), sz, sz]),
+        "mk_dev_kv4_attn": (i32, [C.POINTER(Kv4Cache), i32, vp, sz, sz, vp, sz, f32, sz, vp, vp, vp]),
+        "mk_linear_attn_workspace_bytes": (sz, [sz, sz, sz, sz, sz]),
+        "mk_dev_linear_attn": (i32, [i32, vp, sz, vp, sz, vp, sz, vp, sz, sz, vp, sz, sz, sz, sz, sz, f32, vp, vp, vp, vp, vp]),
+        "mk_dev_linear_attn_step": (i32, [i32, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, sz, f32, vp, vp, vp, vp]),
         "mk_dev_mxfp4_grouped_gemm": (i32, [vp, vp, sz, sz, sz, vp, vp, vp, sz, vp, vp]),
         "mk_dev_mxfp4_grouped_gemm_f32": (i32, [vp, vp, sz, sz, sz, vp, vp, sz, vp, vp]),
         "mk_dev_mxfp4_grouped_gemm_bf16": (i32, [vp, vp, sz, sz, sz, vp, vp, sz, vp, vp]),

@@ -1,0 +1,196 @@
+// RMS norm of every query and key head with the rotation of its position, one pass over the rows.
+//
+//   r = x / sqrt(mean(x^2) + eps) * w        per head row of hd values (w: one row of weights for the queries, one for the keys)
+//   (a, b) -> (a c - b s, a s + b c)         on the rot values from rot_at on; (a, b) = (2 i, 2 i + 1) or (i, i + rot / 2),
+//                                            c, s = table row of the token's position, entry i
+//
+// Everything between the load and the store is f32; a bfloat16 result is rounded once.  A row of hd values lies in LPR
+// lanes, 8 values (one or two 16-byte loads) each: the sum of squares is log2(LPR) exchanges, a pair (i, i + rot / 2) one
+// exchange per value.  A group of LPR lanes keeps the token's table values and the weights in registers and walks
+// ROWS heads of that token, all their loads in flight before the first is used.
+#include "mk_common.h"
+
+namespace {
+
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
+        const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    }
+    static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
+        *(mk_f4 *)p = mk_f4{v[0], v[1], v[2], v[3]};
+        *(mk_f4 *)(p + 4) = mk_f4{v[4], v[5], v[6], v[7]};
+    }
+};
+typedef __bf16 mk_b8 __attribute__((ext_vector_type(8)));
+template <> struct Vec8<__bf16> {
+    static __device__ __forceinline__ void load(const __bf16 *p, float (&v)[8]) {
+        const mk_b8 a = *(const mk_b8 *)p;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+    }
+    static __device__ __forceinline__ void store(__bf16 *p, const float (&v)[8]) {
+        mk_b8 a;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
+        *(mk_b8 *)p = a;
+    }
+};
+
+struct NormRopeArgs {
+    const void *q, *k;
+    void *qo, *ko;
+    size_t qs, ks, qos, kos;  // values from one token's row to the next
+    const float *wq, *wk, *cos, *sin;
+    const int32_t *pos;
+    int n_pos, nh, nkv, hd, rot, rot_at, norm, blocks_q, blocks_per_token;
+    float eps;
+};
+
+template <typename T, int LPR, int ROWS, bool HALVES>
+__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
+    constexpr int GROUPS = 256 / LPR;
+    const int t = blockIdx.x / a.blocks_per_token;
+    int blk = blockIdx.x - t * a.blocks_per_token;
+    const bool is_k = blk >= a.blocks_q;
+    if (is_k) blk -= a.blocks_q;
+    const int heads = is_k ? a.nkv : a.nh;
+    const int p = a.pos ? a.pos[t] : 0;
+    if (p < 0) return;  // a padding row
+    const int l = threadIdx.x % LPR, e0 = l * 8;
+    const bool live = e0 < a.hd;
+    const T *src = is_k ? (const T *)a.k + (size_t)t * a.ks : (const T *)a.q + (size_t)t * a.qs;
+    T *dst = is_k ? (T *)a.ko + (size_t)t * a.kos : (T *)a.qo + (size_t)t * a.qos;
+    const float *wp = is_k ? a.wk : a.wq;
+
+    const int h0 = blk * GROUPS * ROWS + threadIdx.x / LPR;
+    float x[ROWS][8];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int h = h0 + r * GROUPS;
+        if (live && h < heads) {
+            Vec8<T>::load(src + (size_t)h * a.hd + e0, x[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[r][i] = 0.0f;
+        }
+    }
+    float w[8], c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = 1.0f, c[i] = 1.0f, s[i] = 0.0f;
+    if (live && wp) Vec8<float>::load(wp + e0, w);
+    const int ri = e0 - a.rot_at;
+    const bool turned = a.rot && live && ri >= 0 && ri < a.rot;
+    const bool upper = HALVES && ri >= a.rot / 2;
+    if (turned) {
+        if (p < a.n_pos) {
+            const size_t row = (size_t)p * (a.rot / 2);
+            if (HALVES) {
+                const int i0 = upper ? ri - a.rot / 2 : ri;
+                Vec8<float>::load(a.cos + row + i0, c);
+                Vec8<float>::load(a.sin + row + i0, s);
+            } else {
+                const mk_f4 cv = *(const mk_f4 *)(a.cos + row + ri / 2), sv = *(const mk_f4 *)(a.sin + row + ri / 2);
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[i] = cv[i], s[i] = sv[i];
+            }
+        } else {  // the table has no such position: the rotated values are NaN
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = __builtin_nanf(""), s[i] = __builtin_nanf("");
+        }
+        if (HALVES && !upper) {  // lower half: mine * c - partner * s; upper half: mine * c + partner * s
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] = -s[i];
+        }
+    }
+    const int me = threadIdx.x & 63, mate = HALVES && turned ? me + (upper ? -(a.rot / 16) : a.rot / 16) : me;
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int h = h0 + r * GROUPS;
+        float f = 1.0f;
+        if (a.norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[r][i], x[r][i], ss);
+#pragma unroll
+            for (int off = 1; off < LPR; off <<= 1) ss += __shfl_xor(ss, off, MK_WAVE);
+            f = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
+        }
+        float y[8], o[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = x[r][i] * f * w[i];
+        if (HALVES) {
+            if (a.rot) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float other = __shfl(y[i], mate, MK_WAVE);
+                    o[i] = turned ? fmaf(y[i], c[i], other * s[i]) : y[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = y[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                o[2 * i] = turned ? fmaf(y[2 * i], c[i], -(y[2 * i + 1] * s[i])) : y[2 * i];
+                o[2 * i + 1] = turned ? fmaf(y[2 * i], s[i], y[2 * i + 1] * c[i]) : y[2 * i + 1];
+            }
+        }
+        if (live && h < heads) Vec8<T>::store(dst + (size_t)h * a.hd + e0, o);
+    }
+}
+
+template <typename T, int LPR, int ROWS>
+int launch(NormRopeArgs a, size_t n_tok, int halves, hipStream_t st) {
+    constexpr int PER = 256 / LPR * ROWS;
+    a.blocks_q = (a.nh + PER - 1) / PER;
+    a.blocks_per_token = a.blocks_q + (a.nkv + PER - 1) / PER;
+    const size_t grid = n_tok * (size_t)a.blocks_per_token;
+    MK_REQUIRE(grid <= 0x7FFFFFFFull, "too many rows in one call");
+    if (halves)
+        hipLaunchKernelGGL((norm_rope_kernel<T, LPR, ROWS, true>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((norm_rope_kernel<T, LPR, ROWS, false>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    return mk_launch_status("norm_rope");
+}
+
+template <typename T>
+int launch_width(const NormRopeArgs &a, size_t n_tok, int halves, hipStream_t st) {
+    if (a.hd <= 64) return launch<T, 8, 1>(a, n_tok, halves, st);
+    if (a.hd <= 128) return launch<T, 16, 1>(a, n_tok, halves, st);
+    if (a.hd <= 256) return launch<T, 32, 1>(a, n_tok, halves, st);
+    return launch<T, 64, 1>(a, n_tok, halves, st);
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+extern "C" int mk_dev_qk_norm_rope(int dtype, const void *q, size_t q_stride, size_t nh, const void *k, size_t k_stride, size_t nkv, size_t T,
+                                   size_t hd, int norm, const float *wq, const float *wk, float eps, const float *cos, const float *sin,
+                                   size_t n_pos, const int32_t *pos, size_t rot, size_t rot_at, int halves, void *q_out, size_t q_out_stride,
+                                   void *k_out, size_t k_out_stride, void *stream) {
+    MK_REQUIRE(dtype == MK_F32 || dtype == MK_BF16, "dtype must be MK_F32 or MK_BF16");
+    MK_REQUIRE(T == 0 || ((nh == 0 || (q && q_out)) && (nkv == 0 || (k && k_out))), "null pointer");
+    MK_REQUIRE(nh <= 65535 && nkv <= 65535 && T <= 0x7FFFFFFFull && n_pos <= 0x7FFFFFFFull, "size out of range");
+    MK_REQUIRE(hd >= 8 && hd <= 512 && hd % 8 == 0, "head width must be a multiple of 8 up to 512");
+    MK_REQUIRE(rot % 16 == 0 && rot_at % 8 == 0 && rot_at <= hd && rot <= hd - rot_at, "rot must be a multiple of 16, rot_at of 8, both inside the head");
+    MK_REQUIRE(T == 0 || rot == 0 || (cos && sin && pos), "a rotation needs the tables and the positions");
+    MK_REQUIRE(q_stride % 8 == 0 && k_stride % 8 == 0 && q_out_stride % 8 == 0 && k_out_stride % 8 == 0, "token strides must be multiples of 8 values");
+    MK_REQUIRE((nh == 0 || T <= 1 || (q_stride >= nh * hd && q_out_stride >= nh * hd)) &&
+                   (nkv == 0 || T <= 1 || (k_stride >= nkv * hd && k_out_stride >= nkv * hd)),
+               "a token stride is shorter than a token's heads");
+    MK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(q_out) && aligned16(k_out) && aligned16(wq) && aligned16(wk) && aligned16(cos) && aligned16(sin),
+               "pointers must be 16-byte aligned");
+    if (T == 0 || nh + nkv == 0) return MK_OK;
+    NormRopeArgs a;
+    a.q = q, a.k = k, a.qo = q_out, a.ko = k_out;
+    a.qs = q_stride, a.ks = k_stride, a.qos = q_out_stride, a.kos = k_out_stride;
+    a.wq = wq, a.wk = wk, a.cos = cos, a.sin = sin, a.pos = pos;
+    a.n_pos = (int)n_pos, a.nh = (int)nh, a.nkv = (int)nkv, a.hd = (int)hd, a.rot = (int)rot, a.rot_at = (int)rot_at, a.norm = norm ? 1 : 0, a.eps = eps;
+    a.blocks_q = a.blocks_per_token = 0;
+    return dtype == MK_F32 ? launch_width<float>(a, T, halves, (hipStream_t)stream) : launch_width<__bf16>(a, T, halves, (hipStream_t)stream);
+}

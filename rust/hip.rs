@@ -12,7 +12,7 @@
 //! ```
 //!
 //! This file was written against the header and has not been compiled: the build image has no Rust toolchain.
-#![allow(dead_code)]
+#![allow(dead_code, non_snake_case)]
 use std::ffi::CStr;
 use std::os::raw::{c_char, c_int, c_void};
 
@@ -30,6 +30,8 @@ pub const MK_ACT_DS: c_int = 2;
 pub const MK_ROUTER_SOFTMAX: c_int = 0;
 pub const MK_ROUTER_SIGMOID: c_int = 1;
 pub const MK_ROUTER_SQRTSOFTPLUS: c_int = 2;
+pub const MK_F32: c_int = 0;
+pub const MK_BF16: c_int = 1;
 pub const MK_BIN_MAX_DIMS: usize = 8;
 
 /// mk_expert_table: device arrays of per-expert device pointers, indexed by expert id.
@@ -55,6 +57,24 @@ pub struct MkExpertTable {
     pub w1st: *const *const u8,
     pub w3st: *const *const u8,
     pub w2st: *const *const u8,
+}
+
+/// mk_kv4_cache: a KV cache held in 4 bits, device pointers (layout in mk_hip.h).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct MkKv4Cache {
+    pub B: usize,
+    pub nkv: usize,
+    pub dk: usize,
+    pub rope: usize,
+    pub dv: usize,
+    pub cap: usize,
+    pub kq: *mut u8,
+    pub ks: *mut u8,
+    pub vq: *mut u8,
+    pub vs: *mut u8,
+    pub kr: *mut u16,
+    pub lens: *mut i32,
 }
 
 /// mk_bin_entry: one directory entry of an MKIM file (weights::Entry, src/weights.rs:31-37).
@@ -172,6 +192,14 @@ extern "C" {
     pub fn mk_dev_mla_heads_to_f32(kq: *const i8, ks: *const f32, kr: *const f32, vq: *const i8, vs: *const f32, n: usize, nh: usize, nope: usize, rope: usize, vd: usize, hadamard: c_int, k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
     pub fn mk_mla_heads_workspace_bytes(m: usize, nh: usize, nope: usize, vd: usize) -> usize;
     pub fn mk_dev_mla_heads_q8_attn(kq: *const i8, ks: *const f32, kr: *const f32, vq: *const i8, vs: *const f32, pos0: usize, q: *const f32, m: usize, nh: usize, nope: usize, rope: usize, vd: usize, scale: f32, hadamard: c_int, workspace: *mut c_void, out: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn mk_dev_qk_norm_rope(dtype: c_int, q: *const c_void, q_stride: usize, nh: usize, k: *const c_void, k_stride: usize, nkv: usize, T: usize, hd: usize, norm: c_int, wq: *const f32, wk: *const f32, eps: f32, cos: *const f32, sin: *const f32, n_pos: usize, pos: *const i32, rot: usize, rot_at: usize, halves: c_int, q_out: *mut c_void, q_out_stride: usize, k_out: *mut c_void, k_out_stride: usize, stream: *mut c_void) -> c_int;
+    pub fn mk_dev_kv4_append(c: *const MkKv4Cache, dtype: c_int, k_rows: *const c_void, k_stride: usize, v_rows: *const c_void, v_stride: usize, T: usize, cu: *const i32, fresh: c_int, stream: *mut c_void) -> c_int;
+    pub fn mk_dev_kv4_to_f32(c: *const MkKv4Cache, n: usize, k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn mk_kv4_attn_workspace_bytes(c: *const MkKv4Cache, T: usize, nh: usize) -> usize;
+    pub fn mk_dev_kv4_attn(c: *const MkKv4Cache, dtype: c_int, q: *const c_void, q_stride: usize, T: usize, cu: *const i32, nh: usize, scale: f32, max_len: usize, workspace: *mut c_void, out: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mk_linear_attn_workspace_bytes(T: usize, B: usize, nh: usize, dk: usize, dv: usize) -> usize;
+    pub fn mk_dev_linear_attn(dtype: c_int, q: *const c_void, q_stride: usize, k: *const c_void, k_stride: usize, v: *const c_void, v_stride: usize, g: *const f32, g_stride: usize, T: usize, cu: *const i32, B: usize, nh: usize, nkh: usize, dk: usize, dv: usize, scale: f32, state: *const f32, state_out: *mut f32, workspace: *mut c_void, out: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mk_dev_linear_attn_step(dtype: c_int, q: *const c_void, q_stride: usize, k: *const c_void, k_stride: usize, v: *const c_void, v_stride: usize, g: *const f32, g_stride: usize, B: usize, nh: usize, nkh: usize, dk: usize, dv: usize, scale: f32, state: *const f32, state_out: *mut f32, out: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn mk_dev_mxfp4_grouped_gemm(packed_ptrs: *const *const u8, scales_ptrs: *const *const u8, n_groups: usize, rows: usize, cols: usize, codes: *const u8, exps: *const u8, offsets: *const i32, m: usize, out: *mut f32, stream: *mut c_void) -> c_int;
     pub fn mk_dev_mxfp4_grouped_gemm_f32(packed_ptrs: *const *const u8, scales_ptrs: *const *const u8, n_groups: usize, rows: usize, cols: usize, x: *const f32, offsets: *const i32, m: usize, out: *mut f32, stream: *mut c_void) -> c_int;
     pub fn mk_dev_mxfp4_grouped_gemm_bf16(packed_ptrs: *const *const u8, scales_ptrs: *const *const u8, n_groups: usize, rows: usize, cols: usize, x: *const u16, offsets: *const i32, m: usize, out: *mut f32, stream: *mut c_void) -> c_int;
