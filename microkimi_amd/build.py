@@ -8,7 +8,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmk_hip.so")
 SOURCES = ["host.hip", "codec.hip", "gemv_mxfp4.hip", "gemv_q8.hip", "moe.hip", "moe_persist.hip", "mla.hip", "mla_heads.hip", "gemm_mxfp4.hip", "gemm_q8x.hip", "prefill.hip", "front.hip", "weights.hip", "vq1.hip", "quantize.hip",
-           "norm_rope.hip", "kv4.hip", "linear_attn.hip"]
+           "norm_rope.hip", "kv4.hip", "kv4_attn.hip", "linear_attn.hip"]
 
 
 def hipcc():

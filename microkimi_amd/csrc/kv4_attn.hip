@@ -1,0 +1,556 @@
+// Attention over the 4-bit KV cache (kv4.hip writes it).
+#include "mk_mixer.h"
+
+namespace {
+
+constexpr int MAX_SPLITS = 64;
+
+// --------------------------------------------------------------------------------------------------- attention: any width
+
+struct AttnArgs {
+    const void *q;
+    size_t q_stride;
+    void *out;        // [T][nh][dv]
+    float *po;        // partial sums [split][T * nh][dv], unnormalized
+    float *pm, *pl;   // their maxima (of s * log2 e) and sums [split][T * nh]
+    int nh, n_splits, chunk;  // chunk: positions of a split (the last one takes what is left)
+    float scale_log2; // scale * log2(e)
+};
+
+// positions a row may see: 0 ..= the returned one; -1: none; cap and beyond: the cache does not hold them all
+__device__ __forceinline__ int64_t row_limit(const MkKv4 &c, const MkSeqs &s, int b, int t) { return (int64_t)c.lens[b] - (s.at(b + 1) - t); }
+
+// the end of a split's positions when there are n in all
+__device__ __forceinline__ int chunk_end(const AttnArgs &a, int split, int n) { return split + 1 == a.n_splits ? n : min(n, (split + 1) * a.chunk); }
+
+template <typename T> __device__ __forceinline__ void store1(void *out, size_t i, float v) {
+    if constexpr (sizeof(T) == 4) ((float *)out)[i] = v;
+    else ((__bf16 *)out)[i] = (__bf16)v;
+}
+
+constexpr int GT = 256;  // positions of a tile: one a thread
+
+// One workgroup: (row, query head, split).  Scores: a thread takes a position of the tile.  Output: a thread takes 8 values (one
+// dword) of V for every (256 / (dv / 8))-th position of the tile.  Every cache byte is read once per query head, so this is the
+// form for widths that the matrix kernels below do not take.
+template <typename T>
+__global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+    __shared__ float q_l[512 + 64], p_l[GT], red_l[8], acc_l[256 * 9];
+    const int t = blockIdx.x, h = blockIdx.y, split = blockIdx.z, tid = threadIdx.x;
+    const int b = s.of_row(t);
+    if (b < 0) return;
+    const int hk = h / (a.nh / c.nkv), qw = c.dk + c.rope;
+    const int64_t lim64 = row_limit(c, s, b, t);
+    const bool beyond = lim64 >= c.cap;
+    const int n = beyond ? 0 : (int)max(lim64 + 1, (int64_t)0);
+    for (int i = tid; i < qw; i += 256) q_l[i] = (float)((const T *)a.q)[(size_t)t * a.q_stride + (size_t)h * qw + i];
+    const int j0 = split * a.chunk, j1 = chunk_end(a, split, n);
+    if (a.n_splits > 1 && j0 >= j1) return;
+    const size_t base = ((size_t)b * c.nkv + hk) * c.cap;
+    const int cols = c.dv / 8, groups = 256 / cols, col = tid % cols, grp = tid / cols;
+    float m = -INFINITY, l = 0.0f, acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] = 0.0f;
+    __syncthreads();
+    for (int jt = j0; jt < j1; jt += GT) {
+        const int j = jt + tid;
+        float sc = -INFINITY;
+        if (j < j1) {
+            const uint8_t *kp = c.kq + (base + j) * (c.dk / 2), *ksp = c.ks + (base + j) * (c.dk / 32);
+            float sum = 0.0f;
+            for (int g = 0; g < c.dk / 32; g++) {
+                float blk = 0.0f;
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t code = *(const uint32_t *)(kp + g * 16 + w * 4);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) blk = fmaf(mk_e2m1((code >> (4 * i)) & 15u), q_l[g * 32 + w * 8 + i], blk);
+                }
+                sum = fmaf(blk, mk_scale_from_byte(ksp[g]), sum);
+            }
+            for (int i = 0; i < c.rope; i++) sum = fmaf(__uint_as_float((uint32_t)c.kr[((size_t)b * c.cap + j) * c.rope + i] << 16), q_l[c.dk + i], sum);
+            sc = sum * a.scale_log2;
+        }
+        float mx = mk_wave_max(sc);
+        if ((tid & 63) == 0) red_l[tid >> 6] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(fmaxf(red_l[0], red_l[1]), fmaxf(red_l[2], red_l[3])), m);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        const float corr = exp2f(m - ref), p = j < j1 ? exp2f(sc - ref) : 0.0f;
+        p_l[tid] = p;
+        const float sum = mk_wave_sum(p);
+        if ((tid & 63) == 0) red_l[4 + (tid >> 6)] = sum;
+        __syncthreads();
+        l = l * corr + ((red_l[4] + red_l[5]) + (red_l[6] + red_l[7]));
+        m = mx;
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc[i] *= corr;
+        if (grp < groups) {
+            const int nj = min(GT, j1 - jt);
+            for (int i = grp; i < nj; i += groups) {
+                const size_t row = base + jt + i;
+                const uint32_t code = *(const uint32_t *)(c.vq + row * (c.dv / 2) + col * 4);
+                const float w = p_l[i] * mk_scale_from_byte(c.vs[row * (c.dv / 32) + col / 4]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[e] = fmaf(mk_e2m1((code >> (4 * e)) & 15u), w, acc[e]);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc_l[tid * 9 + i] = acc[i];
+    __syncthreads();
+    for (int d = tid; d < c.dv; d += 256) {
+        float o = 0.0f;
+        for (int g = 0; g < groups; g++) o += acc_l[(g * cols + d / 8) * 9 + d % 8];
+        const size_t row = (size_t)t * a.nh + h;
+        if (a.n_splits > 1) a.po[((size_t)split * s.T * a.nh + row) * c.dv + d] = o;
+        else store1<T>(a.out, row * c.dv + d, beyond ? __builtin_nanf("") : n == 0 ? 0.0f : o / l);
+    }
+    if (a.n_splits > 1 && tid == 0) {
+        a.pm[(size_t)split * s.T * a.nh + (size_t)t * a.nh + h] = m;
+        a.pl[(size_t)split * s.T * a.nh + (size_t)t * a.nh + h] = l;
+    }
+}
+
+// ------------------------------------------------------------------------------- attention on the matrix cores, pieces
+//
+// Both kernels below compute S^T = K Q^T and O^T = V^T P^T: a query column (row of the call x head of the kv head's group) is a
+// column n = lane % 16 of every tile, so its running maximum and sum live in that lane, and the scores of a tile, as the
+// instruction returns them (rows 4 g + j, g = lane / 16), ARE the second product's operand once the positions of a 32-step are
+// taken in the order {4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3}: a sum over positions has no order of its own.  In the same way
+// the sum over the K width takes the values (DK / 4) g .. of lane group g: a lane reads DK / 8 consecutive bytes of one
+// position, which is one block (one scale byte) at DK = 128.
+//
+// 4-bit values become bfloat16 exactly (two significant bits, and the exponent of an f32), so the products are exact in f32.
+// f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as PT terms: three
+// for f32 results, two (17 bits) for bfloat16 results, whose own rounding is 2^-8.
+constexpr float LOG2E = 1.44269504088896340736f;
+
+template <typename T> struct Terms;
+template <> struct Terms<float> { static constexpr int Q = 3, P = 3; };
+template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2; };
+
+__device__ __forceinline__ mk_f4 mfma(mk_b8 a, mk_b8 b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// x as the sum of N bfloat16 terms, largest first
+template <int N> __device__ __forceinline__ void split8(const float (&x)[8], mk_b8 (&t)[N]) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const __bf16 h = (__bf16)r[i];
+            t[k][i] = h;
+            if (k + 1 < N) r[i] -= (float)h;
+        }
+    }
+}
+
+// eight 4-bit values of a block with scale sc -> bfloat16
+__device__ __forceinline__ mk_b8 fp4x8(uint32_t w, float sc) {
+    const mk_b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
+    const mk_b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
+    return mk_b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The columns of a workgroup: number `idx` in the list of tiles of CT columns of all sequences (a sequence with m rows and group G has
+// m * G columns).  Every wave finds it for itself.  false: past the end of the list.
+__device__ __forceinline__ bool find_tile(const MkSeqs &s, int G, int CT, int idx, int &b, int &tile) {
+    if (!s.cu) {
+        const int per = (s.T / s.B * G + CT - 1) / CT;
+        b = idx / per;
+        tile = idx - b * per;
+        return b < s.B;
+    }
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+        const int mine = b0 + lane;
+        int n = mine < s.B ? (max(s.at(mine + 1) - s.at(mine), 0) * G + CT - 1) / CT : 0;
+        int sum = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(sum, off, MK_WAVE);
+            if (lane >= off) sum += o;
+        }
+        const int total = __shfl(sum, 63, MK_WAVE);
+        if (idx < total) {
+            const uint64_t hit = __ballot(sum > idx);
+            const int l = __builtin_ctzll(hit);
+            b = b0 + l;
+            tile = idx - __shfl(sum - n, l, MK_WAVE);
+            return true;
+        }
+        idx -= total;
+    }
+    return false;
+}
+
+// A query column.
+struct Column {
+    int t, h, lim;  // row of the call, query head, last position it may see (-1: none)
+    bool live, beyond;
+};
+__device__ __forceinline__ Column column(const MkKv4 &c, const MkSeqs &s, int G, int hk, int b, int idx) {
+    Column o;
+    const int first = s.at(b), m = max(s.at(b + 1) - first, 0), i = idx / G;
+    o.live = i < m;
+    o.t = first + i;
+    o.h = hk * G + idx - i * G;
+    const int64_t lim = (int64_t)c.lens[b] - m + i;
+    o.beyond = o.live && lim >= c.cap;
+    o.lim = o.live && !o.beyond && lim >= 0 ? (int)lim : -1;
+    return o;
+}
+__device__ __forceinline__ int columns_max(int v) {  // over the 16 columns of the wave
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) v = max(v, __shfl_xor(v, off, MK_WAVE));
+    return v;
+}
+__device__ __forceinline__ int columns_min(int v) {
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) v = min(v, __shfl_xor(v, off, MK_WAVE));
+    return v;
+}
+
+// The query operand: step st of lane group g is values (DK / 4) g + 8 st .. of the K width, then (R / 4) g + 8 (st - NS) .. of the tail.
+template <typename T, int DK, int R>
+__device__ __forceinline__ void load_query(const AttnArgs &a, const Column &o, int g, mk_b8 (&qf)[DK / 32 + R / 32][Terms<T>::Q]) {
+    const T *row = (const T *)a.q + (size_t)o.t * a.q_stride + (size_t)o.h * (DK + R);
+#pragma unroll
+    for (int st = 0; st < DK / 32 + R / 32; st++) {
+        const int d = st < DK / 32 ? DK / 4 * g + 8 * st : DK + R / 4 * g + 8 * (st - DK / 32);
+        float x[8];
+        if (o.live) {
+            mk_load8(row + d, x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.0f;
+        }
+        split8<Terms<T>::Q>(x, qf[st]);
+    }
+}
+
+// ------------------------------------------------------------------------- few query columns: every wave its own positions
+//
+// One workgroup: (tile of 16 query columns, kv head, chunk of the context).  Its four waves take the chunk's steps of 32 positions
+// in turn, straight from global memory into registers (no LDS, no barrier), the next step's bytes asked for while this one is
+// computed; at the end the four partial results meet in LDS.
+//   K  lane (n, g): position n of 16, DK / 8 bytes from (DK / 4) g on: one load; a wave's load is 16 whole rows
+//   V  lane (n, g): the DV / 16 values from (DV / 16) n on of its 8 positions; the values of one dimension at 8 positions are put
+//      together with byte permutes and are the first operand of tile j = dimension (DV / 16) n + j
+template <int BYTES> struct Raw;
+template <> struct Raw<2> { typedef uint16_t type; };
+template <> struct Raw<4> { typedef uint32_t type; };
+template <> struct Raw<8> { typedef mk_u2 type; };
+template <> struct Raw<16> { typedef mk_v4u type; };
+
+template <int DK, int R, int DV> struct Step {
+    static constexpr int KD = DK / 32, KL = DK == 256 ? 2 : 1;  // dwords of a lane's K bytes; 16-byte loads
+    typedef typename Raw<DK == 256 ? 16 : DK / 8>::type KT;
+    typedef typename Raw<DV / 32>::type VT;
+    KT k[2][KL];
+    uint16_t ks[2];
+    mk_b8 kr[2][R ? R / 32 : 1];
+    VT v[8];
+    uint8_t vs[8];
+
+    // positions j .. j + 31; those past `last` are read as `last`
+    template <bool FULL>
+    __device__ __forceinline__ void load(const MkKv4 &c, size_t row0, size_t kr0, int j, int last, int n, int g) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int p = FULL ? j + 16 * s + n : min(j + 16 * s + n, last);
+            const uint8_t *kp = c.kq + row0 * (DK / 2) + (size_t)(uint32_t)(p * (DK / 2) + g * (DK / 8));
+#pragma unroll
+            for (int i = 0; i < KL; i++) k[s][i] = *(const KT *)(kp + 16 * i);
+            const uint8_t *sp = c.ks + row0 * (DK / 32) + (size_t)(uint32_t)(p * (DK / 32));
+            if constexpr (DK == 256) ks[s] = *(const uint16_t *)(sp + 2 * g);
+            else if constexpr (DK == 128) ks[s] = sp[g];
+            else ks[s] = sp[g / 2];
+#pragma unroll
+            for (int i = 0; i < R / 32; i++) kr[s][i] = *(const mk_b8 *)(c.kr + (kr0 + p) * R + R / 4 * g + 8 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int q = j + 4 * g + (i & 3) + 16 * (i >> 2), p = FULL ? q : min(q, last);
+            v[i] = *(const VT *)(c.vq + row0 * (DV / 2) + (size_t)(uint32_t)(p * (DV / 2) + n * (DV / 32)));
+            vs[i] = c.vs[row0 * (DV / 32) + (size_t)(uint32_t)(p * (DV / 32) + n / (512 / DV))];
+        }
+    }
+    __device__ __forceinline__ uint32_t kword(int s, int i) const {
+        if constexpr (DK == 256) return k[s][i / 4][i % 4];
+        else return k[s][0][i];
+    }
+    __device__ __forceinline__ uint32_t vword(int i, int w) const {
+        if constexpr (DV == 256) return v[i][w];
+        else return v[i];
+    }
+};
+
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// First operands of V^T for the DV / 16 tiles: element i of tile j = value (DV / 16) n + j at the lane's position i.
+template <int DK, int R, int DV>
+__device__ __forceinline__ void value_tiles(const Step<DK, R, DV> &x, mk_b8 (&vt)[DV / 16]) {
+    constexpr int W = DV / 32;  // pairs of values of a position
+    uint32_t pr[8][W];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float sc = scale_of(x.vs[i]);
+#pragma unroll
+        for (int w = 0; w < (W + 3) / 4; w++) {
+            const uint32_t d = x.vword(i, w);
+            pr[i][4 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 0));
+            pr[i][4 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 1));
+            if constexpr (W >= 4) {
+                pr[i][4 * w + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 2));
+                pr[i][4 * w + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 3));
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < DV / 16; j++) {
+        mk_v4u o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1][j / 2], pr[2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+        vt[j] = __builtin_bit_cast(mk_b8, o);
+    }
+}
+
+template <typename T, int DK, int R, int DV>
+__global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+    constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::P, LD = DV + 4;
+    __shared__ float o_l[4][16][LD], m_l[4][16], l_l[4][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.y, split = blockIdx.z, G = a.nh / c.nkv;
+    int b, tile;
+    if (!find_tile(s, G, 16, blockIdx.x, b, tile)) return;
+    const Column col = column(c, s, G, hk, b, tile * 16 + n);
+    const int top = columns_max(col.lim), low = columns_min(col.live ? col.lim : 0x7FFFFFFF);
+    const int j0 = split * a.chunk, j1 = chunk_end(a, split, top + 1);
+    if (a.n_splits > 1 && j0 >= j1) return;  // nothing here: the merge knows which chunks a row has
+    const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
+
+    float m = -INFINITY, l = 0.0f;
+    mk_f4 o[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) o[j] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    int j = j0 + 32 * wave;
+    if (j < j1) {
+        mk_b8 qf[NS + NR][QT];
+        Step<DK, R, DV> cur;
+        if (j + 32 <= j1) cur.template load<true>(c, row0, kr0, j, 0, n, g);
+        else cur.template load<false>(c, row0, kr0, j, j1 - 1, n, g);
+        load_query<T, DK, R>(a, col, g, qf);
+        while (true) {
+            const int nj = j + 128;
+            Step<DK, R, DV> nxt;
+            if (nj + 32 <= j1) nxt.template load<true>(c, row0, kr0, nj, 0, n, g);
+            else if (nj < j1) nxt.template load<false>(c, row0, kr0, nj, j1 - 1, n, g);
+            // scores
+            float sc[8];
+#pragma unroll
+            for (int ss = 0; ss < 2; ss++) {
+                mk_f4 acc = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < NS; st++) {
+                    const float k_sc = scale_of(DK == 256 ? (st < 4 ? cur.ks[ss] & 255u : cur.ks[ss] >> 8) : cur.ks[ss]);
+                    const mk_b8 kf = fp4x8(cur.kword(ss, st), k_sc);
+#pragma unroll
+                    for (int t = 0; t < QT; t++) acc = mfma(kf, qf[st][t], acc);
+                }
+#pragma unroll
+                for (int st = 0; st < NR; st++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) acc = mfma(cur.kr[ss][st], qf[NS + st][t], acc);
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[4 * ss + i] = acc[i] * a.scale_log2;
+            }
+            if (j + 31 > low) {  // some column does not see all of these positions
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (j + 4 * g + (i & 3) + 16 * (i >> 2) > min(col.lim, j1 - 1)) sc[i] = -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+            mx = mk_rows_max(mx);
+            if (__any(mx > m)) {
+                mx = fmaxf(mx, m);
+                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+                m = mx;
+                l *= corr;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t][i] *= corr;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sc[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
+            l += ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
+            mk_b8 pf[PT], vt[NT];
+            split8<PT>(sc, pf);
+            value_tiles(cur, vt);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < PT; k++) o[t] = mfma(vt[t], pf[k], o[t]);
+            if (nj >= j1) break;
+            cur = nxt;
+            j = nj;
+        }
+        l = mk_rows_sum(l);
+    }
+    // the waves' partial results: lane (n, g) holds values NT (4 g + i) + t of column n
+    if (g == 0) m_l[wave][n] = m, l_l[wave][n] = l;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int t = 0; t < NT; t += 4) *(mk_f4 *)&o_l[wave][n][NT * (4 * g + i) + t] = mk_f4{o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]};
+    __syncthreads();
+    const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * (DV / 16);  // 16 threads a column
+    const Column out = column(c, s, G, hk, b, tile * 16 + oc);
+    if (!out.live) return;
+    float mw[4], mx = -INFINITY, den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) mx = fmaxf(mx, m_l[w][oc]);
+    // (a query that is not finite gives NaN sums, whatever the maximum says)
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int w = 0; w < 4; w++) mw[w] = __builtin_amdgcn_exp2f(m_l[w][oc] - ref), den = fmaf(l_l[w][oc], mw[w], den);
+    float r[DV / 16];
+#pragma unroll
+    for (int i = 0; i < DV / 16; i++) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) v = fmaf(o_l[w][oc][od + i], mw[w], v);
+        r[i] = v;
+    }
+    const size_t row = (size_t)out.t * a.nh + out.h;
+    if (a.n_splits > 1) {
+        const size_t at = (size_t)split * s.T * a.nh + row;
+        float *po = a.po + at * DV + od;
+#pragma unroll
+        for (int i = 0; i < DV / 16; i += 4) *(mk_f4 *)(po + i) = mk_f4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+        if (od == 0) a.pm[at] = mx, a.pl[at] = den;
+    } else {
+        const float inv = out.beyond ? __builtin_nanf("") : out.lim < 0 ? 0.0f : 1.0f / den;
+#pragma unroll
+        for (int i = 0; i < DV / 16; i++) store1<T>(a.out, row * DV + od + i, r[i] * inv);
+    }
+}
+
+// ------------------------------------------------------------------------------------------- the chunks' results together
+
+// One wave: (row, head).  Lane i has the statistics of chunk i: weights 2^(m_i - max), one division.
+template <typename T>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+    static_assert(MAX_SPLITS <= MK_WAVE, "one lane a chunk");
+    const size_t rows = (size_t)s.T * a.nh, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63, t = (int)(row / a.nh), b = s.of_row(t);
+    if (b < 0) return;
+    const int64_t lim = row_limit(c, s, b, t);
+    const int used = lim < 0 || lim >= c.cap ? 0 : min((int)lim / a.chunk + 1, a.n_splits);
+    const float empty = lim < 0 ? 0.0f : __builtin_nanf("");
+    const float m = lane < used ? a.pm[lane * rows + row] : -INFINITY, l = lane < used ? a.pl[lane * rows + row] : 0.0f;
+    const float mx = mk_wave_max(m), ref = mx == -INFINITY ? 0.0f : mx;
+    const float w = __builtin_amdgcn_exp2f(m - ref), den = mk_wave_sum(l * w);
+    for (int d = 4 * lane; d < c.dv; d += 4 * MK_WAVE) {
+        mk_f4 num = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < used; i++) {
+            const mk_f4 o = *(const mk_f4 *)(a.po + (i * rows + row) * c.dv + d);
+            const float wi = mk_readlane(w, i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) num[k] = fmaf(o[k], wi, num[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) store1<T>(a.out, row * c.dv + d + k, used ? num[k] / den : empty);
+    }
+}
+
+// Positions of a chunk: `pairs` workgroups walk `len` positions each.  About 4096 chunks in all (16 a compute unit, so that ragged
+// sequences even out), of 256 to 1024 positions (below, the merge costs more than it spreads; above, one long sequence is a tail),
+// at most MAX_SPLITS of them.
+void plan(AttnArgs &a, size_t pairs, size_t len) {
+    size_t chunk = (pairs * len / 4096 + 127) / 128 * 128;
+    chunk = chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+    const size_t least = (len + MAX_SPLITS - 1) / MAX_SPLITS;
+    if (chunk < least) chunk = (least + 127) / 128 * 128;
+    a.chunk = (int)chunk;
+    a.n_splits = (int)((len + chunk - 1) / chunk);
+}
+
+// the widths the matrix kernels are built for: (K, tail, V)
+bool matrix_widths(const mk_kv4_cache *c) {
+    return c->dk == c->dv ? (c->dk == 64 || c->dk == 128 || c->dk == 256) && (c->rope == 0 || c->rope == 64) : false;
+}
+size_t column_tiles(const mk_kv4_cache *c, size_t T, const int32_t *cu, size_t group, size_t ct) {
+    return cu ? T * group / ct + c->B : c->B * ((T / c->B * group + ct - 1) / ct);
+}
+
+template <typename T, int D>
+void launch_few(const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.rope) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, 64, D>), grid, dim3(256), 0, st, v, s, a);
+    else hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, 0, D>), grid, dim3(256), 0, st, v, s, a);
+}
+template <typename T>
+void launch_few(const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.dk == 64) launch_few<T, 64>(grid, st, v, s, a);
+    else if (v.dk == 128) launch_few<T, 128>(grid, st, v, s, a);
+    else launch_few<T, 256>(grid, st, v, s, a);
+}
+
+}  // namespace
+
+extern "C" size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh) {
+    if (!c || !T || !nh) return 256;
+    const size_t n = c->cap <= 256 ? 1 : MAX_SPLITS < (c->cap + 255) / 256 ? MAX_SPLITS : (c->cap + 255) / 256;
+    return n <= 1 ? 256 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
+}
+
+extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_stride, size_t T, const int32_t *cu, size_t nh, float scale,
+                               size_t max_len, void *workspace, void *out, void *stream) {
+    int st = mk_kv4_check(c);
+    if (st != MK_OK || (st = mk_kv4_check_rows(c, dtype, T, cu)) != MK_OK) return st;
+    MK_REQUIRE(nh >= 1 && nh <= 65535 && nh % c->nkv == 0, "the query heads must be a multiple of the kv heads");
+    if (T == 0) return MK_OK;
+    MK_REQUIRE(q && out && workspace, "null pointer");
+    MK_REQUIRE(q_stride % 8 == 0 && mk_aligned16(q) && mk_aligned16(out) && ((uintptr_t)workspace & 255) == 0,
+               "q and out must be 16-byte, the workspace 256-byte aligned, the query stride a multiple of 8 values");
+    MK_REQUIRE(T == 1 || q_stride >= nh * (c->dk + c->rope), "the query stride is shorter than a token's heads");
+    MK_REQUIRE(T * nh <= 0x7FFFFFFFull, "too many query rows in one call");
+    AttnArgs a;
+    a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = scale * LOG2E;
+    const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
+    const bool matrix = matrix_widths(c);
+    const size_t tiles = matrix ? column_tiles(c, T, cu, group, 16) : T * group;
+    plan(a, tiles * c->nkv, len);
+    uint8_t *w = (uint8_t *)workspace;
+    a.po = (float *)w;
+    w += mk_align_up((size_t)a.n_splits * T * nh * c->dv * 4, 256);
+    a.pm = (float *)w;
+    w += mk_align_up((size_t)a.n_splits * T * nh * 4, 256);
+    a.pl = (float *)w;
+    const MkSeqs s{cu, (int)T, (int)c->B};
+    const MkKv4 v = mk_kv4_view(c);
+    hipStream_t hs = (hipStream_t)stream;
+    if (matrix) {
+        const dim3 grid((unsigned)tiles, (unsigned)c->nkv, (unsigned)a.n_splits);
+        if (dtype == MK_F32) launch_few<float>(grid, hs, v, s, a);
+        else launch_few<__bf16>(grid, hs, v, s, a);
+    } else {
+        const dim3 grid((unsigned)T, (unsigned)nh, (unsigned)a.n_splits);
+        if (dtype == MK_F32) hipLaunchKernelGGL(kv4_attn_any_kernel<float>, grid, dim3(256), 0, hs, v, s, a);
+        else hipLaunchKernelGGL(kv4_attn_any_kernel<__bf16>, grid, dim3(256), 0, hs, v, s, a);
+    }
+    if ((st = mk_launch_status("kv4_attn")) != MK_OK) return st;
+    if (a.n_splits > 1) {
+        const unsigned blocks = (unsigned)((T * nh + 3) / 4);
+        if (dtype == MK_F32) hipLaunchKernelGGL(kv4_merge_kernel<float>, dim3(blocks), dim3(256), 0, hs, v, s, a);
+        else hipLaunchKernelGGL(kv4_merge_kernel<__bf16>, dim3(blocks), dim3(256), 0, hs, v, s, a);
+        return mk_launch_status("kv4_merge");
+    }
+    return MK_OK;
+}

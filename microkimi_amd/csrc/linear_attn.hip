@@ -5,11 +5,10 @@
 //
 // g_t is a log decay per token and head, or one constant per head; g = -inf empties the state.  Query / key heads may be fewer
 // than value heads (head h reads key head h / (nh / nkh)).  Sequences of a batch lie one behind the other.
-#include "mk_common.h"
+#include "mk_mixer.h"
 
 namespace {
 
-typedef __bf16 mk_b8 __attribute__((ext_vector_type(8)));
 
 struct LinArgs {
     const void *q, *k, *v;
@@ -105,7 +104,6 @@ int launch_token(const LinArgs &a, hipStream_t st) {
     return mk_launch_status("linear_token");
 }
 
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, const void *v, size_t vs, const float *g, size_t gs, size_t T, size_t B,
                  size_t nh, size_t nkh, size_t dk, size_t dv, const float *state, const float *state_out, const void *out) {
@@ -116,7 +114,7 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
     MK_REQUIRE(g && state_out && (T == 0 || (q && k && v && out)), "null pointer");
     MK_REQUIRE(qs % 8 == 0 && ks % 8 == 0 && vs % 8 == 0, "token strides must be multiples of 8 values");
     MK_REQUIRE(T <= 1 || (qs >= nkh * dk && ks >= nkh * dk && vs >= nh * dv && (gs == 0 || gs >= nh)), "a token stride is shorter than a token's heads");
-    MK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(state) && aligned16(state_out), "pointers must be 16-byte aligned");
+    MK_REQUIRE(mk_aligned16(q) && mk_aligned16(k) && mk_aligned16(v) && mk_aligned16(out) && mk_aligned16(state) && mk_aligned16(state_out), "pointers must be 16-byte aligned");
     return MK_OK;
 }
 

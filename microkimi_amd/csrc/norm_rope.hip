@@ -8,7 +8,7 @@
 // lanes, 8 values (one or two 16-byte loads) each: the sum of squares is log2(LPR) exchanges, a pair (i, i + rot / 2) one
 // exchange per value.  A group of LPR lanes keeps the token's table values and the weights in registers and walks
 // ROWS heads of that token, all their loads in flight before the first is used.
-#include "mk_common.h"
+#include "mk_mixer.h"
 
 namespace {
 
@@ -24,7 +24,6 @@ template <> struct Vec8<float> {
         *(mk_f4 *)(p + 4) = mk_f4{v[4], v[5], v[6], v[7]};
     }
 };
-typedef __bf16 mk_b8 __attribute__((ext_vector_type(8)));
 template <> struct Vec8<__bf16> {
     static __device__ __forceinline__ void load(const __bf16 *p, float (&v)[8]) {
         const mk_b8 a = *(const mk_b8 *)p;
@@ -165,7 +164,6 @@ int launch_width(const NormRopeArgs &a, size_t n_tok, int halves, hipStream_t st
     return launch<T, 64, 1>(a, n_tok, halves, st);
 }
 
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
@@ -183,7 +181,7 @@ extern "C" int mk_dev_qk_norm_rope(int dtype, const void *q, size_t q_stride, si
     MK_REQUIRE((nh == 0 || T <= 1 || (q_stride >= nh * hd && q_out_stride >= nh * hd)) &&
                    (nkv == 0 || T <= 1 || (k_stride >= nkv * hd && k_out_stride >= nkv * hd)),
                "a token stride is shorter than a token's heads");
-    MK_REQUIRE(aligned16(q) && aligned16(k) && aligned16(q_out) && aligned16(k_out) && aligned16(wq) && aligned16(wk) && aligned16(cos) && aligned16(sin),
+    MK_REQUIRE(mk_aligned16(q) && mk_aligned16(k) && mk_aligned16(q_out) && mk_aligned16(k_out) && mk_aligned16(wq) && mk_aligned16(wk) && mk_aligned16(cos) && mk_aligned16(sin),
                "pointers must be 16-byte aligned");
     if (T == 0 || nh + nkv == 0) return MK_OK;
     NormRopeArgs a;
