@@ -4,6 +4,7 @@
 namespace {
 
 constexpr int MAX_SPLITS = 64;
+constexpr int MAX_CT = 128;  // the most query columns that a workgroup of any form below takes
 
 // --------------------------------------------------------------------------------------------------- attention: any width
 
@@ -14,7 +15,8 @@ struct AttnArgs {
     float *po;        // partial sums [split][T * nh][dv], unnormalized
     float *pm, *pl;   // their maxima (of s * log2 e) and sums [split][T * nh]
     int nh, n_splits, chunk;  // chunk: positions of a split (the last one takes what is left)
-    float scale_log2; // scale * log2(e)
+    float scale_log2; // |scale| * log2(e)
+    float sign;       // the scale's sign, taken by the query
 };
 
 // positions a row may see: 0 ..= the returned one; -1: none; cap and beyond: the cache does not hold them all
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, At
                 sum = fmaf(blk, mk_scale_from_byte(ksp[g]), sum);
             }
             for (int i = 0; i < c.rope; i++) sum = fmaf(__uint_as_float((uint32_t)c.kr[((size_t)b * c.cap + j) * c.rope + i] << 16), q_l[c.dk + i], sum);
-            sc = sum * a.scale_log2;
+            sc = sum * (a.sign * a.scale_log2);
         }
         float mx = mk_wave_max(sc);
         if ((tid & 63) == 0) red_l[tid >> 6] = mx;
@@ -217,121 +219,138 @@ __device__ __forceinline__ int columns_min(int v) {
 // The query operand: step st of lane group g is values (DK / 4) g + 8 st .. of the K width, then (R / 4) g + 8 (st - NS) .. of the tail.
 template <typename T, int DK, int R>
 __device__ __forceinline__ void load_query(const AttnArgs &a, const Column &o, int g, mk_b8 (&qf)[DK / 32 + R / 32][Terms<T>::Q]) {
-    const T *row = (const T *)a.q + (size_t)o.t * a.q_stride + (size_t)o.h * (DK + R);
+    constexpr int N = DK / 32 + R / 32;
+    // (a column without a row reads row 0 and drops it: all loads are in flight together)
+    const T *row = (const T *)a.q + (o.live ? (size_t)o.t * a.q_stride + (size_t)o.h * (DK + R) : 0);
+    float x[N][8];
 #pragma unroll
-    for (int st = 0; st < DK / 32 + R / 32; st++) {
-        const int d = st < DK / 32 ? DK / 4 * g + 8 * st : DK + R / 4 * g + 8 * (st - DK / 32);
-        float x[8];
-        if (o.live) {
-            mk_load8(row + d, x);
-        } else {
+    for (int st = 0; st < N; st++) mk_load8(row + (st < DK / 32 ? DK / 4 * g + 8 * st : DK + R / 4 * g + 8 * (st - DK / 32)), x[st]);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.0f;
-        }
-        split8<Terms<T>::Q>(x, qf[st]);
+    for (int st = 0; st < N; st++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[st][i] = o.live ? x[st][i] * a.sign : 0.0f;
+        split8<Terms<T>::Q>(x[st], qf[st]);
     }
 }
 
 // ------------------------------------------------------------------------- few query columns: every wave its own positions
 //
-// One workgroup: (tile of 16 query columns, kv head, chunk of the context).  Its four waves take the chunk's steps of 32 positions
-// in turn, straight from global memory into registers (no LDS, no barrier), the next step's bytes asked for while this one is
-// computed; at the end the four partial results meet in LDS.
+// One workgroup: (tile of 16 query columns, kv head, chunk of the context), the heads fastest: neighbours in the grid, which go to
+// the eight XCDs in turn, then have the same length (with the sequences fastest a long one's workgroups all met on one XCD:
+// 75 us instead of 35 for 32 ragged sequences).  Its four waves take the chunk's steps of 32 positions
+// in turn, straight from global memory into registers (no LDS, no barrier); at the end the four partial results meet in LDS.
 //   K  lane (n, g): position n of 16, DK / 8 bytes from (DK / 4) g on: one load; a wave's load is 16 whole rows
 //   V  lane (n, g): the DV / 16 values from (DV / 16) n on of its 8 positions; the values of one dimension at 8 positions are put
 //      together with byte permutes and are the first operand of tile j = dimension (DV / 16) n + j
+// A step's K registers are asked for again (for the next step) as soon as the scores are formed, its V registers as soon as they
+// are converted: the loads fly over the other half of the step and no register is copied.  Addresses are a scalar base (the
+// step) plus a lane offset that never changes.  A chunk's last step that is not whole is moved back to end with it; the
+// positions it then sees twice, or that lie behind the sequence, are masked.
 template <int BYTES> struct Raw;
 template <> struct Raw<2> { typedef uint16_t type; };
 template <> struct Raw<4> { typedef uint32_t type; };
 template <> struct Raw<8> { typedef mk_u2 type; };
 template <> struct Raw<16> { typedef mk_v4u type; };
 
-template <int DK, int R, int DV> struct Step {
-    static constexpr int KD = DK / 32, KL = DK == 256 ? 2 : 1;  // dwords of a lane's K bytes; 16-byte loads
-    typedef typename Raw<DK == 256 ? 16 : DK / 8>::type KT;
-    typedef typename Raw<DV / 32>::type VT;
-    KT k[2][KL];
-    uint16_t ks[2];
-    mk_b8 kr[2][R ? R / 32 : 1];
-    VT v[8];
-    uint8_t vs[8];
+template <typename V> __device__ __forceinline__ V ldg(const uint8_t *base, uint32_t off) {
+    const MK_GLOBAL uint8_t *b = (const MK_GLOBAL uint8_t *)base;
+    return *(const MK_GLOBAL V *)(b + off);
+}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+template <typename P> __device__ __forceinline__ const uint8_t *uniform(const P *p) { return mk_uniform_ptr((const uint8_t *)p); }
 
-    // positions j .. j + 31; those past `last` are read as `last`
-    template <bool FULL>
-    __device__ __forceinline__ void load(const MkKv4 &c, size_t row0, size_t kr0, int j, int last, int n, int g) {
+template <int DK, int R> struct KStep {
+    static constexpr int KL = DK == 256 ? 2 : 1;  // 16-byte loads
+    typedef typename Raw<DK == 256 ? 16 : DK / 8>::type KT;
+    KT k[2][KL];
+    uint32_t ks[2];
+    mk_b8 kr[2][R ? R / 32 : 1];
+    // 32 positions from j on; kq, ks, kr: the rows of the head's position 0
+    __device__ __forceinline__ void load(const uint8_t *kqp, const uint8_t *ksp, const uint8_t *krp, int j, int n, int g) {
+        const uint8_t *kj = kqp + (size_t)j * (DK / 2), *sj = ksp + (size_t)j * (DK / 32), *rj = krp + (size_t)j * (R * 2);
+        const uint32_t ko = n * (DK / 2) + g * (DK / 8), so = n * (DK / 32) + (DK == 256 ? 2 * g : DK == 128 ? g : g / 2), ro = n * (R * 2) + g * (R / 2);
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const int p = FULL ? j + 16 * s + n : min(j + 16 * s + n, last);
-            const uint8_t *kp = c.kq + row0 * (DK / 2) + (size_t)(uint32_t)(p * (DK / 2) + g * (DK / 8));
 #pragma unroll
-            for (int i = 0; i < KL; i++) k[s][i] = *(const KT *)(kp + 16 * i);
-            const uint8_t *sp = c.ks + row0 * (DK / 32) + (size_t)(uint32_t)(p * (DK / 32));
-            if constexpr (DK == 256) ks[s] = *(const uint16_t *)(sp + 2 * g);
-            else if constexpr (DK == 128) ks[s] = sp[g];
-            else ks[s] = sp[g / 2];
+            for (int i = 0; i < KL; i++) k[s][i] = ldg<KT>(kj, ko + (8 * DK * s + 16 * i));
+            if constexpr (DK == 256) ks[s] = ldg<uint16_t>(sj, so + DK / 2 * s);
+            else ks[s] = ldg<uint8_t>(sj, so + DK / 2 * s);
 #pragma unroll
-            for (int i = 0; i < R / 32; i++) kr[s][i] = *(const mk_b8 *)(c.kr + (kr0 + p) * R + R / 4 * g + 8 * i);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int q = j + 4 * g + (i & 3) + 16 * (i >> 2), p = FULL ? q : min(q, last);
-            v[i] = *(const VT *)(c.vq + row0 * (DV / 2) + (size_t)(uint32_t)(p * (DV / 2) + n * (DV / 32)));
-            vs[i] = c.vs[row0 * (DV / 32) + (size_t)(uint32_t)(p * (DV / 32) + n / (512 / DV))];
+            for (int i = 0; i < R / 32; i++) kr[s][i] = ldg<mk_b8>(rj, ro + (32 * R * s + 16 * i));
         }
     }
-    __device__ __forceinline__ uint32_t kword(int s, int i) const {
+    __device__ __forceinline__ uint32_t word(int s, int i) const {
         if constexpr (DK == 256) return k[s][i / 4][i % 4];
         else return k[s][0][i];
     }
-    __device__ __forceinline__ uint32_t vword(int i, int w) const {
-        if constexpr (DV == 256) return v[i][w];
-        else return v[i];
+    __device__ __forceinline__ float scale(int s, int st) const {
+        if constexpr (DK == 256) return scale_of(st < 4 ? ks[s] & 255u : ks[s] >> 8);
+        else return scale_of(ks[s]);
     }
 };
 
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-
-// First operands of V^T for the DV / 16 tiles: element i of tile j = value (DV / 16) n + j at the lane's position i.
-template <int DK, int R, int DV>
-__device__ __forceinline__ void value_tiles(const Step<DK, R, DV> &x, mk_b8 (&vt)[DV / 16]) {
-    constexpr int W = DV / 32;  // pairs of values of a position
-    uint32_t pr[8][W];
+template <int DV> struct VStep {
+    typedef typename Raw<DV / 32>::type VT;
+    typedef typename Raw<DV == 64 ? 4 : DV / 32>::type VL;
+    VL v[8];
+    uint32_t vs[8];  // (whole registers: a byte of a packed one would be waited for at its load)
+    __device__ __forceinline__ void load(const uint8_t *vqp, const uint8_t *vsp, int j, int n, int g) {
+        const uint8_t *vj = vqp + (size_t)j * (DV / 2), *sj = vsp + (size_t)j * (DV / 32);
+        const uint32_t vo = 4 * g * (DV / 2) + n * (DV / 32), so = 4 * g * (DV / 32) + n / (512 / DV);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float sc = scale_of(x.vs[i]);
-#pragma unroll
-        for (int w = 0; w < (W + 3) / 4; w++) {
-            const uint32_t d = x.vword(i, w);
-            pr[i][4 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 0));
-            pr[i][4 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 1));
-            if constexpr (W >= 4) {
-                pr[i][4 * w + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 2));
-                pr[i][4 * w + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 3));
-            }
+        for (int i = 0; i < 8; i++) {
+            const int p = (i & 3) + 16 * (i >> 2);
+            v[i] = ldg<VT>(vj, vo + p * (DV / 2));
+            vs[i] = ldg<uint8_t>(sj, so + p * (DV / 32));
         }
     }
-#pragma unroll
-    for (int j = 0; j < DV / 16; j++) {
-        mk_v4u o;
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1][j / 2], pr[2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-        vt[j] = __builtin_bit_cast(mk_b8, o);
+    __device__ __forceinline__ uint32_t word(int i, int w) const {
+        if constexpr (DV == 256) return v[i][w];
+        else return v[i];
     }
-}
+    // first operand of V^T for tile j: element i = value (DV / 16) n + j at the lane's position i
+    __device__ __forceinline__ void tiles(mk_b8 (&vt)[DV / 16]) const {
+        constexpr int W = DV / 32;  // pairs of values of a position
+        uint32_t pr[8][W];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float sc = scale_of(vs[i]);
+#pragma unroll
+            for (int w = 0; w < (W + 3) / 4; w++) {
+                const uint32_t d = word(i, w);
+                pr[i][4 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 0));
+                pr[i][4 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 1));
+                if constexpr (W >= 4) {
+                    pr[i][4 * w + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 2));
+                    pr[i][4 * w + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 3));
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < DV / 16; j++) {
+            mk_v4u o;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1][j / 2], pr[2 * i][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+            vt[j] = __builtin_bit_cast(mk_b8, o);
+        }
+    }
+};
 
 template <typename T, int DK, int R, int DV>
 __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
     constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::P, LD = DV + 4;
     __shared__ float o_l[4][16][LD], m_l[4][16], l_l[4][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.y, split = blockIdx.z, G = a.nh / c.nkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % c.nkv, split = blockIdx.x / c.nkv % a.n_splits, G = a.nh / c.nkv;
     int b, tile;
-    if (!find_tile(s, G, 16, blockIdx.x, b, tile)) return;
+    if (!find_tile(s, G, 16, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
     const Column col = column(c, s, G, hk, b, tile * 16 + n);
-    const int top = columns_max(col.lim), low = columns_min(col.live ? col.lim : 0x7FFFFFFF);
+    const int top = __builtin_amdgcn_readfirstlane(columns_max(col.lim));
+    const int low = __builtin_amdgcn_readfirstlane(columns_min(col.live ? col.lim : 0x7FFFFFFF));
     const int j0 = split * a.chunk, j1 = chunk_end(a, split, top + 1);
     if (a.n_splits > 1 && j0 >= j1) return;  // nothing here: the merge knows which chunks a row has
-    const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
 
     float m = -INFINITY, l = 0.0f;
     mk_f4 o[NT];
@@ -339,16 +358,18 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
     for (int j = 0; j < NT; j++) o[j] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
     int j = j0 + 32 * wave;
     if (j < j1) {
+        const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
+        const uint8_t *kqp = uniform(c.kq + row0 * (DK / 2)), *ksp = uniform(c.ks + row0 * (DK / 32)), *vqp = uniform(c.vq + row0 * (DV / 2)),
+                      *vsp = uniform(c.vs + row0 * (DV / 32)), *krp = R ? uniform(c.kr + kr0 * R) : nullptr;
         mk_b8 qf[NS + NR][QT];
-        Step<DK, R, DV> cur;
-        if (j + 32 <= j1) cur.template load<true>(c, row0, kr0, j, 0, n, g);
-        else cur.template load<false>(c, row0, kr0, j, j1 - 1, n, g);
+        KStep<DK, R> ks;
+        VStep<DV> vs;
+        int at = max(min(j, j1 - 32), 0);  // (a cache has room for 32 positions at least)
         load_query<T, DK, R>(a, col, g, qf);
+        ks.load(kqp, ksp, krp, at, n, g);
+        vs.load(vqp, vsp, at, n, g);
         while (true) {
-            const int nj = j + 128;
-            Step<DK, R, DV> nxt;
-            if (nj + 32 <= j1) nxt.template load<true>(c, row0, kr0, nj, 0, n, g);
-            else if (nj < j1) nxt.template load<false>(c, row0, kr0, nj, j1 - 1, n, g);
+            const int nj = j + 128, nat = max(min(nj, j1 - 32), 0);
             // scores
             float sc[8];
 #pragma unroll
@@ -356,28 +377,36 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
                 mk_f4 acc = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int st = 0; st < NS; st++) {
-                    const float k_sc = scale_of(DK == 256 ? (st < 4 ? cur.ks[ss] & 255u : cur.ks[ss] >> 8) : cur.ks[ss]);
-                    const mk_b8 kf = fp4x8(cur.kword(ss, st), k_sc);
+                    const mk_b8 kf = fp4x8(ks.word(ss, st), ks.scale(ss, st));
 #pragma unroll
                     for (int t = 0; t < QT; t++) acc = mfma(kf, qf[st][t], acc);
                 }
 #pragma unroll
                 for (int st = 0; st < NR; st++)
 #pragma unroll
-                    for (int t = 0; t < QT; t++) acc = mfma(cur.kr[ss][st], qf[NS + st][t], acc);
+                    for (int t = 0; t < QT; t++) acc = mfma(ks.kr[ss][st], qf[NS + st][t], acc);
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[4 * ss + i] = acc[i] * a.scale_log2;
+                for (int i = 0; i < 4; i++) sc[4 * ss + i] = acc[i];
             }
-            if (j + 31 > low) {  // some column does not see all of these positions
+            ks.load(kqp, ksp, krp, nat, n, g);  // (past the last step: that step again, so that the loads in flight are always the same)
+            if (at < j || at + 31 > low) {  // positions seen before, or that some column does not see
+                const int last = min(col.lim, j1 - 1);
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (j + 4 * g + (i & 3) + 16 * (i >> 2) > min(col.lim, j1 - 1)) sc[i] = -INFINITY;
+                for (int i = 0; i < 8; i++) {
+                    const int p = at + 4 * g + (i & 3) + 16 * (i >> 2);
+                    if (p < j || p > last) sc[i] = -INFINITY;
+                }
+                if (at + 32 > j1) {  // a sequence shorter than a step: what lies behind it may hold any scale byte
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (at + 4 * g + (i & 3) + 16 * (i >> 2) >= j1) vs.vs[i] = 0;
+                }
             }
             float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
             mx = mk_rows_max(mx);
             if (__any(mx > m)) {
                 mx = fmaxf(mx, m);
-                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * a.scale_log2);
                 m = mx;
                 l *= corr;
 #pragma unroll
@@ -385,25 +414,26 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
 #pragma unroll
                     for (int i = 0; i < 4; i++) o[t][i] *= corr;
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
+            const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2;
 #pragma unroll
-            for (int i = 0; i < 8; i++) sc[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
+            for (int i = 0; i < 8; i++) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2, -ref));
             l += ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
             mk_b8 pf[PT], vt[NT];
             split8<PT>(sc, pf);
-            value_tiles(cur, vt);
+            vs.tiles(vt);
+            vs.load(vqp, vsp, nat, n, g);
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int k = 0; k < PT; k++) o[t] = mfma(vt[t], pf[k], o[t]);
             if (nj >= j1) break;
-            cur = nxt;
+            at = nat;
             j = nj;
         }
         l = mk_rows_sum(l);
     }
     // the waves' partial results: lane (n, g) holds values NT (4 g + i) + t of column n
-    if (g == 0) m_l[wave][n] = m, l_l[wave][n] = l;
+    if (g == 0) m_l[wave][n] = m == -INFINITY ? m : m * a.scale_log2, l_l[wave][n] = l;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -459,27 +489,45 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnA
     const float w = __builtin_amdgcn_exp2f(m - ref), den = mk_wave_sum(l * w);
     for (int d = 4 * lane; d < c.dv; d += 4 * MK_WAVE) {
         mk_f4 num = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < used; i++) {
-            const mk_f4 o = *(const mk_f4 *)(a.po + (i * rows + row) * c.dv + d);
-            const float wi = mk_readlane(w, i);
+        for (int i0 = 0; i0 < used; i0 += 8) {  // eight loads in flight
+            mk_f4 o[8];
 #pragma unroll
-            for (int k = 0; k < 4; k++) num[k] = fmaf(o[k], wi, num[k]);
+            for (int i = 0; i < 8; i++)
+                if (i0 + i < used) o[i] = *(const mk_f4 *)(a.po + ((size_t)(i0 + i) * rows + row) * c.dv + d);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i0 + i < used) {
+                    const float wi = mk_readlane(w, i0 + i);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) num[k] = fmaf(o[i][k], wi, num[k]);
+                }
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) store1<T>(a.out, row * c.dv + d + k, used ? num[k] / den : empty);
     }
 }
 
-// Positions of a chunk: `pairs` workgroups walk `len` positions each.  About 4096 chunks in all (16 a compute unit, so that ragged
-// sequences even out), of 256 to 1024 positions (below, the merge costs more than it spreads; above, one long sequence is a tail),
-// at most MAX_SPLITS of them.
+// Positions of a chunk, when `pairs` (column tile, kv head) walk `len` positions each.  About 1024 chunks fill the 256 compute units; below
+// 256 positions (two steps a wave) a chunk is start and end only, above 1024 one long sequence among short ones is a tail (32
+// ragged sequences: 38.6 / 35.4 / 41.1 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
+// costs what the split saves (96 heads, 1024 positions: 13.2 us, in four chunks 10.3 + 4.0 us).
 void plan(AttnArgs &a, size_t pairs, size_t len) {
-    size_t chunk = (pairs * len / 4096 + 127) / 128 * 128;
-    chunk = chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+    size_t chunk = (pairs * len / 1024 + 127) / 128 * 128;
+    chunk = len <= 1024 ? len : chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
     const size_t least = (len + MAX_SPLITS - 1) / MAX_SPLITS;
     if (chunk < least) chunk = (least + 127) / 128 * 128;
     a.chunk = (int)chunk;
     a.n_splits = (int)((len + chunk - 1) / chunk);
+}
+// The most chunks that plan() makes for `pairs` or more and any length up to cap: chunks of 256 until pairs * len reaches 1024 * 256, then
+// at most 1024 / pairs (and one that is not whole) of them, from chunks of 1024 on len / 1024.
+size_t most_splits(size_t pairs, size_t cap) {
+    if (cap <= 1024) return 1;
+    size_t n = (1024 + pairs - 1) / pairs + 1;
+    const size_t by_len = (cap + 1023) / 1024;
+    n = n < by_len ? by_len : n;
+    n = n < (cap + 255) / 256 ? n : (cap + 255) / 256;
+    return n < MAX_SPLITS ? n : MAX_SPLITS;
 }
 
 // the widths the matrix kernels are built for: (K, tail, V)
@@ -505,8 +553,10 @@ void launch_few(const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &
 }  // namespace
 
 extern "C" size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh) {
-    if (!c || !T || !nh) return 256;
-    const size_t n = c->cap <= 256 ? 1 : MAX_SPLITS < (c->cap + 255) / 256 ? MAX_SPLITS : (c->cap + 255) / 256;
+    if (!c || !T || !nh || !c->nkv || !c->cap) return 256;
+    // no form of the call has fewer (column tile, kv head) pairs than this
+    const size_t cols = T * (nh / c->nkv ? nh / c->nkv : 1), pairs = c->nkv * (cols / MAX_CT ? cols / MAX_CT : 1);
+    const size_t n = most_splits(pairs, c->cap);
     return n <= 1 ? 256 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
 }
 
@@ -522,9 +572,9 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     MK_REQUIRE(T == 1 || q_stride >= nh * (c->dk + c->rope), "the query stride is shorter than a token's heads");
     MK_REQUIRE(T * nh <= 0x7FFFFFFFull, "too many query rows in one call");
     AttnArgs a;
-    a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = scale * LOG2E;
+    a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
-    const bool matrix = matrix_widths(c);
+    const bool matrix = matrix_widths(c) && c->cap >= 32;
     const size_t tiles = matrix ? column_tiles(c, T, cu, group, 16) : T * group;
     plan(a, tiles * c->nkv, len);
     uint8_t *w = (uint8_t *)workspace;
@@ -537,7 +587,8 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     const MkKv4 v = mk_kv4_view(c);
     hipStream_t hs = (hipStream_t)stream;
     if (matrix) {
-        const dim3 grid((unsigned)tiles, (unsigned)c->nkv, (unsigned)a.n_splits);
+        MK_REQUIRE(tiles * c->nkv * a.n_splits <= 0x7FFFFFFFull, "too many query rows in one call");
+        const dim3 grid((unsigned)(tiles * c->nkv * a.n_splits));
         if (dtype == MK_F32) launch_few<float>(grid, hs, v, s, a);
         else launch_few<__bf16>(grid, hs, v, s, a);
     } else {
