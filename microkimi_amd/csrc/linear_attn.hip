@@ -105,6 +105,414 @@ int launch_token(const LinArgs &a, hipStream_t st) {
 }
 
 
+// ------------------------------------------------------------------------------------------------ blocks of 64 tokens
+//
+// With b_i the sum of the log decays of a block up to its token i (S: the state before the block, m: its last token):
+//   o_i = scale * ( e^{b_i} S^T q_i + sum_{j <= i} e^{b_i - b_j} (q_i . k_j) v_j )
+//   S'  = e^{b_m} S + sum_j (e^{b_m - b_j} v_j) k_j^T
+// which is all matrix products, and every exponent of the decays is a difference of sums of the same block: formed in 64 bits, so that
+// no large sum cancels, it is never positive for log decays that are not (a log decay below -200 counts as -200: e^-200 is 0).
+//
+// One workgroup: a run of blocks of (value head, sequence), its four waves a quarter of dv each.  The state stays in registers
+// across the blocks, as the matrix instruction returns it: tile (kt, t) of S = rows 16 kt + 4 g + j, column n (lane = 16 g + n).  Two
+// such tiles ARE an operand of the next product once the sum over dk takes its terms in the order {4 g .. , 16 + 4 g ..}; the same
+// holds for the block's scores and the sum over its tokens.  So the waves exchange only the scores (each computes those of 16
+// query tokens), through LDS in operand order.
+//   scores   A = K rows, B = Q rows               -> (key, query), weighted by the decay, masked, to LDS
+//   out      A = S^T, B = Q^T; times e^{b_i}; A = V^T, B = scores     -> (dv, token)
+//   state    A = K^T, B = weighted V^T            -> (dk, dv)
+// bfloat16 rows: S and the weighted scores are rounded to bfloat16 for the products of the output (whose own rounding is as large);
+// the state itself is f32 through and through, so its weighted values enter in three bfloat16 terms (24 bits).
+// f32 rows: the same on the f32 matrix instruction.
+constexpr int CH = 64;
+
+typedef float mk_f8v __attribute__((ext_vector_type(8)));
+template <typename T> struct Op;
+template <> struct Op<__bf16> {
+    typedef mk_b8 F;
+    static constexpr int PAD = 8, TERMS = 3;
+    static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ bool finite(const mk_v4u &r) {  // of a 16-byte piece of a row
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ok &= (r[i] & 0x7F80u) != 0x7F80u && (r[i] & 0x7F800000u) != 0x7F800000u;
+        return ok;
+    }
+};
+template <> struct Op<float> {
+    typedef mk_f8v F;
+    static constexpr int PAD = 4, TERMS = 1;
+    static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ bool finite(const mk_v4u &r) {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ok &= (r[i] & 0x7F800000u) != 0x7F800000u;
+        return ok;
+    }
+};
+// two result tiles (or any 8 values) as an operand
+template <typename T> __device__ __forceinline__ typename Op<T>::F operand(const mk_f4 &lo, const mk_f4 &hi) {
+    typename Op<T>::F f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = (T)lo[i], f[4 + i] = (T)hi[i];
+    return f;
+}
+// values 8 consecutive of a row
+__device__ __forceinline__ mk_b8 row8(const __bf16 *p) { return *(const mk_b8 *)p; }
+__device__ __forceinline__ mk_f8v row8(const float *p) {
+    const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 4);
+    return mk_f8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+// values 4 + 4 of a row, 16 apart
+typedef __bf16 mk_b4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ mk_b8 row44(const __bf16 *p) {
+    const mk_b4 a = *(const mk_b4 *)p, b = *(const mk_b4 *)(p + 16);
+    return mk_b8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+__device__ __forceinline__ mk_f8v row44(const float *p) {
+    const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 16);
+    return mk_f8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+// a transposed operand of a tile in LDS [token][LD]: lane (g, n) gets column col(n) of the tokens 32 ks + 4 g .. + 3 and 16 further; the
+// columns of the 16 lanes of a group are four runs of four, run r at cols + RUN * r
+template <int LD, int RUN> __device__ __forceinline__ mk_b8 column8(const __bf16 *tile, int ks, int cols, int g, int n) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const __bf16 *p = tile + (32 * ks + 4 * g + (n >> 2)) * LD + cols + RUN * (n & 3);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p);
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p + 16 * LD));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(mk_b8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+template <int LD, int RUN> __device__ __forceinline__ mk_f8v column8(const float *tile, int ks, int cols, int g, int n) {
+    mk_f8v f;
+    const float *p = tile + (32 * ks + 4 * g) * LD + cols + RUN * (n >> 2) + (n & 3);
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = p[((i & 3) + 16 * (i >> 2)) * LD];
+    return f;
+}
+
+struct LinSeg {
+    int n_seg;
+    mk_f4 *local;   // [b][h][segment][DK / 16 * NT][256]: local states, then the states before each segment
+    float *decay;   // [b][h][segment]: e^{sum of the segment's log decays}
+};
+// blocks of segment seg of a sequence with n tokens
+__device__ __forceinline__ void segment(int n, int n_seg, int seg, int &c0, int &c1) {
+    const int nch = (n + CH - 1) / CH, per = (nch + n_seg - 1) / n_seg;
+    c0 = min(seg * per, nch);
+    c1 = min(c0 + per, nch);
+}
+// dv column of (lane, tile t) within the state: a wave's quarter, 8 consecutive values in the two tiles of a lane group
+template <int NT> __device__ __forceinline__ int state_col(int wave, int n, int t) { return NT == 2 ? 32 * wave + 8 * (n >> 2) + 4 * t + (n & 3) : 16 * wave + n; }
+
+// inclusive sum over the wave in 64 bits
+__device__ __forceinline__ double wave_scan(double v, int lane) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(v, off, MK_WAVE);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+template <typename T, int DK, int DV, bool OUT>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kernel(LinArgs a, LinSeg sg) {
+    typedef typename Op<T>::F F;
+    constexpr int NT = DV / 64, KT = DK / 16, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, RUN = NT == 2 ? 8 : 4;
+    constexpr int E = 16 / sizeof(T), KP = CH * DK / E / 256, VP = CH * DV / E / 256;  // values of a 16-byte piece; pieces a thread moves
+    __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LK : 8];
+    __shared__ F p_l[OUT ? 6 : 1][64];
+    __shared__ double b_l[CH];
+    __shared__ float w_l[CH], e_l[CH], last_l;
+    __shared__ int bad_l;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int h = blockIdx.x % a.nh, seg = blockIdx.x / a.nh % sg.n_seg, b = blockIdx.x / a.nh / sg.n_seg, hk = h / (a.nh / a.nkh);
+    const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0);
+    int c0, c1;
+    segment(len, sg.n_seg, seg, c0, c1);
+    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV;
+    if (c0 >= c1 && sg.n_seg > 1) return;
+    mk_f4 S[KT][NT];
+    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT * NT) * 256 + threadIdx.x;
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            S[kt][t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (OUT && sg.n_seg > 1) {
+                S[kt][t] = mine[(kt * NT + t) * 256];
+            } else if (OUT && a.state) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) S[kt][t][j] = a.state[sbase + (size_t)(16 * kt + 4 * g + j) * DV + state_col<NT>(wave, n, t)];
+            }
+        }
+    const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * DV;
+    mk_v4u kr[KP], vr[VP], qr[OUT ? KP : 1];
+    float gr;
+    auto fetch = [&](int c) {  // the block's rows into registers; behind the sequence: zeros, and no decay
+        const int first = c * CH;
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            const int at = i * 256 + threadIdx.x, r = first + at / (DK / E), d = at % (DK / E) * E;
+            const size_t row = (size_t)(t0 + min(r, len - 1));
+            const bool in = r < len;
+            const mk_v4u x = *(const mk_v4u *)(kp + row * a.ks + d);
+            kr[i] = in ? x : mk_v4u{0, 0, 0, 0};
+            if constexpr (OUT) {
+                const mk_v4u y = *(const mk_v4u *)(qp + row * a.qs + d);
+                qr[i] = in ? y : mk_v4u{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            const int at = i * 256 + threadIdx.x, r = first + at / (DV / E), d = at % (DV / E) * E;
+            const mk_v4u x = *(const mk_v4u *)(vp + (size_t)(t0 + min(r, len - 1)) * a.vs + d);
+            vr[i] = r < len ? x : mk_v4u{0, 0, 0, 0};
+        }
+        const float x = a.g[a.gs ? (size_t)(t0 + min(first + lane, len - 1)) * a.gs + h : h];
+        gr = first + lane < len ? (x < -200.0f ? -200.0f : x) : 0.0f;
+    };
+    if (c0 < c1) fetch(c0);
+    double total = 0.0;
+    if (threadIdx.x == 0) bad_l = 0;
+    for (int c = c0; c < c1; c++) {
+        __syncthreads();
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < KP; i++) {
+            const int at = i * 256 + threadIdx.x, r = at / (DK / E), d = at % (DK / E) * E;
+            *(mk_v4u *)&k_l[r * LK + d] = kr[i];
+            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + d] = qr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            const int at = i * 256 + threadIdx.x, r = at / (DV / E), d = at % (DV / E) * E;
+            *(mk_v4u *)&v_l[r * LV + d] = vr[i];
+            ok &= Op<T>::finite(vr[i]);
+        }
+        if (OUT && !ok) bad_l = c + 1;
+        if (wave == 0) {
+            const double s = wave_scan((double)gr, lane), end = __shfl(s, 63, MK_WAVE);
+            b_l[lane] = s;
+            w_l[lane] = expf((float)(end - s));
+            e_l[lane] = expf((float)s);
+            if (lane == 0) last_l = expf((float)end);
+            total += end;
+        }
+        __syncthreads();
+        if (c + 1 < c1) fetch(c + 1);
+        if constexpr (OUT) {
+            // scores of the wave's 16 query tokens
+            F qf[DK / 32];
+#pragma unroll
+            for (int s = 0; s < DK / 32; s++) qf[s] = row8(&q_l[(16 * wave + n) * LK + 32 * s + 8 * g]);
+            const double bq = b_l[16 * wave + n];
+            for (int s2 = 0; s2 <= wave / 2; s2++) {
+                mk_f4 pt[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int i = 2 * s2 + u;
+                    pt[u] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (i <= wave) {
+#pragma unroll
+                        for (int s = 0; s < DK / 32; s++) pt[u] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[u]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int key = 16 * i + 4 * g + j;
+                            pt[u][j] = key <= 16 * wave + n ? pt[u][j] * expf((float)(bq - b_l[key])) : 0.0f;
+                        }
+                    }
+                }
+                p_l[s2 == 0 ? wave : 2 + wave][lane] = operand<T>(pt[0], pt[1]);  // (second half: queries 32 .. 63 only)
+            }
+            __syncthreads();
+        }
+        F vt[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) vt[t][ks] = column8<LV, RUN>(v_l, ks, DV / 4 * wave + 4 * t * (NT - 1), g, n);
+        if constexpr (OUT) {
+            const bool plain = bad_l == c + 1;  // a value that is not finite: 0 times it must not reach earlier tokens
+            F sf[NT][DK / 32];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int s = 0; s < DK / 32; s++) sf[t][s] = operand<T>(S[2 * s][t], S[2 * s + 1][t]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                F qb[DK / 32];
+#pragma unroll
+                for (int s = 0; s < DK / 32; s++) qb[s] = row44(&q_l[(16 * j + n) * LK + 32 * s + 4 * g]);
+                mk_f4 o[NT];
+                const float e = e_l[16 * j + n];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    o[t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < DK / 32; s++) o[t] = Op<T>::mma(sf[t][s], qb[s], o[t]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t][i] *= e;
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        o[t] = Op<T>::mma(vt[t][0], p_l[j][lane], o[t]);
+                        if (j >= 2) o[t] = Op<T>::mma(vt[t][1], p_l[2 + j][lane], o[t]);
+                    }
+                } else {
+                    const int tok = 16 * j + n;
+                    for (int key = 0; key <= tok; key++) {
+                        const int r = key & 31;
+                        const float p = (float)p_l[key < 32 ? j : 2 + j][16 * ((r & 15) >> 2) + n][4 * (r >> 4) + (r & 3)];
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[t][i] = fmaf(p, (float)v_l[key * LV + state_col<NT>(wave, 4 * g + i, t)], o[t][i]);
+                    }
+                }
+                const int tok = c * CH + 16 * j + n;
+                if (tok < len) {
+                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + state_col<NT>(wave, 4 * g, 0);
+                    if constexpr (NT == 2) {
+                        const mk_f4 lo = o[0] * a.scale, hi = o[1] * a.scale;
+                        if constexpr (sizeof(T) == 4) *(mk_f4 *)dst = lo, *(mk_f4 *)(dst + 4) = hi;
+                        else *(mk_b8 *)dst = operand<T>(lo, hi);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) dst[i] = (T)(o[0][i] * a.scale);
+                    }
+                }
+            }
+        }
+        // the state behind the block
+        if (!OUT || sg.n_seg == 1 || c + 1 < c1) {
+            const float end = last_l;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) S[kt][t][j] *= end;
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                F wv[NT][Op<T>::TERMS];
+                float w[8];
+                *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[32 * ks + 4 * g];
+                *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[32 * ks + 16 + 4 * g];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float r[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) r[i] = (float)vt[t][ks][i] * w[i];
+#pragma unroll
+                    for (int k = 0; k < Op<T>::TERMS; k++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            wv[t][k][i] = (T)r[i];
+                            r[i] -= (float)wv[t][k][i];
+                        }
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++) {
+                    const F kf = column8<LK, 4>(k_l, ks, 16 * kt, g, n);
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int k = 0; k < Op<T>::TERMS; k++) S[kt][t] = Op<T>::mma(kf, wv[t][k], S[kt][t]);
+                }
+            }
+        }
+    }
+    if (OUT && sg.n_seg > 1) return;
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if constexpr (OUT) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) a.state_out[sbase + (size_t)(16 * kt + 4 * g + j) * DV + state_col<NT>(wave, n, t)] = S[kt][t][j];
+            } else {
+                mine[(kt * NT + t) * 256] = S[kt][t];
+            }
+        }
+    if (!OUT && threadIdx.x == 0) sg.decay[bh * sg.n_seg + seg] = expf((float)total);
+}
+
+// Between the two passes over the segments: local states -> the states before each segment, and the state behind the last.  One
+// workgroup: a quarter of the register tiles of (head, sequence).
+template <int DK, int DV>
+__global__ __launch_bounds__(256) void linear_carry_kernel(LinArgs a, LinSeg sg) {
+    constexpr int NT = DV / 64, TILES = DK / 16 * NT;
+    const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV;
+    const int len = max(a.at(b + 1) - a.at(b), 0);
+    const int tile = blockIdx.x, kt = tile / NT, t = tile % NT;
+    mk_f4 S = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    const size_t at = sbase + (size_t)(16 * kt + 4 * g) * DV + state_col<NT>(wave, n, t);
+    if (a.state) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) S[j] = a.state[at + (size_t)j * DV];
+    }
+    mk_f4 *p = sg.local + (bh * sg.n_seg * TILES + tile) * 256 + threadIdx.x;
+    for (int s0 = 0; s0 < sg.n_seg; s0 += 4) {
+        mk_f4 L[4];
+        float E[4];
+        bool has[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int c0 = 0, c1 = 0;
+            if (s0 + i < sg.n_seg) segment(len, sg.n_seg, s0 + i, c0, c1);
+            has[i] = c0 < c1;
+            if (has[i]) L[i] = p[(size_t)(s0 + i) * TILES * 256], E[i] = sg.decay[bh * sg.n_seg + s0 + i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (has[i]) {
+                p[(size_t)(s0 + i) * TILES * 256] = S;
+#pragma unroll
+                for (int j = 0; j < 4; j++) S[j] = fmaf(E[i], S[j], L[i][j]);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) a.state_out[at + (size_t)j * DV] = S[j];
+}
+
+// Segments that a sequence is cut into: without them a (sequence, head) is one workgroup; with them the keys and values are read
+// twice (local states first, then the outputs from the right states).  As many as fill the device: 2 workgroups a compute unit.
+constexpr int MAX_SEG = 32;
+int segments(size_t T, size_t B, size_t nh) {
+    const size_t blocks = (T / B + CH - 1) / CH, heads = B * nh;
+    size_t n = 512 / heads;
+    n = n < blocks / 2 ? n : blocks / 2;
+    n = n < MAX_SEG ? n : MAX_SEG;
+    return n < 2 ? 1 : (int)n;
+}
+bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv == 64 || dv == 128); }
+
+template <typename T, int DK, int DV>
+int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
+    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B));
+    int e;
+    if (sg.n_seg > 1) {
+        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, false>), grid, dim3(256), 0, st, a, sg);
+        if ((e = mk_launch_status("linear_block")) != MK_OK) return e;
+        hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16 * (DV / 64), (unsigned)a.nh, (unsigned)a.B), dim3(256), 0, st, a, sg);
+        if ((e = mk_launch_status("linear_carry")) != MK_OK) return e;
+    }
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, true>), grid, dim3(256), 0, st, a, sg);
+    return mk_launch_status("linear_block");
+}
+template <typename T>
+int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
+    if (a.dk == 64) return a.dv == 64 ? launch_blocks<T, 64, 64>(a, sg, st) : launch_blocks<T, 64, 128>(a, sg, st);
+    return a.dv == 64 ? launch_blocks<T, 128, 64>(a, sg, st) : launch_blocks<T, 128, 128>(a, sg, st);
+}
+
 int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, const void *v, size_t vs, const float *g, size_t gs, size_t T, size_t B,
                  size_t nh, size_t nkh, size_t dk, size_t dv, const float *state, const float *state_out, const void *out) {
     MK_REQUIRE(dtype == MK_F32 || dtype == MK_BF16, "dtype must be MK_F32 or MK_BF16");
@@ -121,8 +529,9 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
 }  // namespace
 
 extern "C" size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv) {
-    (void)T, (void)B, (void)nh, (void)dk, (void)dv;
-    return 256;
+    if (!B || !nh || !block_widths(dk, dv)) return 256;
+    const size_t n = (size_t)segments(T, B, nh);
+    return n == 1 ? 256 : B * nh * n * dk * dv * 4 + mk_align_up(B * nh * n * 4, 256);
 }
 
 extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
@@ -133,7 +542,12 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     MK_REQUIRE(cu || T % B == 0, "without cu every sequence has the same number of tokens");
     MK_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, "the workspace must be 256-byte aligned");
     const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out};
-    return dtype == MK_F32 ? launch_token<float>(a, (hipStream_t)stream) : launch_token<__bf16>(a, (hipStream_t)stream);
+    hipStream_t hs = (hipStream_t)stream;
+    if (!block_widths(dk, dv)) return dtype == MK_F32 ? launch_token<float>(a, hs) : launch_token<__bf16>(a, hs);
+    LinSeg sg{segments(T, B, nh), (mk_f4 *)workspace, nullptr};
+    sg.decay = (float *)((uint8_t *)workspace + B * nh * sg.n_seg * dk * dv * 4);
+    MK_REQUIRE((size_t)nh * sg.n_seg * B <= 0x7FFFFFFFull, "too many heads and sequences in one call");
+    return dtype == MK_F32 ? launch_blocks<float>(a, sg, hs) : launch_blocks<__bf16>(a, sg, hs);
 }
 
 extern "C" int mk_dev_linear_attn_step(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride,
