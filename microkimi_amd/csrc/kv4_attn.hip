@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, At
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <typename T> struct Terms;
-template <> struct Terms<float> { static constexpr int Q = 3, P = 3; };
-template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2; };
+template <> struct Terms<float> { static constexpr int Q = 3, P = 3, PM = 3; };
+template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2, PM = 2; };
 
 __device__ __forceinline__ mk_f4 mfma(mk_b8 a, mk_b8 b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -471,6 +471,233 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
     }
 }
 
+// ----------------------------------------------------------------------- many query columns: the workgroup shares K and V
+//
+// One workgroup: (tile of 64 NB query columns, kv head, chunk of the context), 64 positions a step.  Each wave turns a quarter of the
+// step's bytes into bfloat16 operands in LDS (as in the kernel above, so no transposed read is needed) and multiplies all of them
+// with its own 16 NB columns; the next step's bytes are on their way meanwhile.  A K operand read from LDS serves NB products.
+// A wave's share of a step of 64 positions: the K rows of 16 of them; the V rows of 32 of them, half of the dimensions.  Positions past
+// `last` are read as `last`.
+template <int DK, int R> struct KQuarter {
+    static constexpr int KL = DK == 256 ? 2 : 1;
+    typedef typename Raw<DK == 256 ? 16 : DK / 8>::type KT;
+    KT k[KL];
+    uint32_t ks;
+    mk_b8 kr[R ? R / 32 : 1];
+    __device__ __forceinline__ void load(const uint8_t *kqp, const uint8_t *ksp, const uint8_t *krp, int j, int last, int n, int g) {
+        const uint32_t p = min(j + n, last);
+#pragma unroll
+        for (int i = 0; i < KL; i++) k[i] = ldg<KT>(kqp, p * (DK / 2) + (g * (DK / 8) + 16 * i));
+        if constexpr (DK == 256) ks = ldg<uint16_t>(ksp, p * (DK / 32) + 2 * g);
+        else ks = ldg<uint8_t>(ksp, p * (DK / 32) + (DK == 128 ? g : g / 2));
+#pragma unroll
+        for (int i = 0; i < R / 32; i++) kr[i] = ldg<mk_b8>(krp, p * (R * 2) + (g * (R / 2) + 16 * i));
+    }
+    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int lane) const {
+#pragma unroll
+        for (int st = 0; st < DK / 32; st++) {
+            uint32_t w;
+            if constexpr (DK == 256) w = k[st / 4][st % 4];
+            else w = k[0][st];
+            dst[st][lane] = fp4x8(w, scale_of(DK == 256 ? (st < 4 ? ks & 255u : ks >> 8) : ks));
+        }
+#pragma unroll
+        for (int i = 0; i < R / 32; i++) dst[DK / 32 + i][lane] = kr[i];
+    }
+};
+template <> struct Raw<1> { typedef uint8_t type; };
+template <int DV> struct VQuarter {
+    typedef typename Raw<DV / 64>::type VT;
+    uint32_t v[8], vs[8];
+    __device__ __forceinline__ void load(const uint8_t *vqp, const uint8_t *vsp, int j, int last, int part, int n, int g) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t p = min(j + 4 * g + (i & 3) + 16 * (i >> 2), last);
+            v[i] = ldg<VT>(vqp, p * (DV / 2) + (n * (DV / 32) + part * (DV / 64)));
+            vs[i] = ldg<uint8_t>(vsp, p * (DV / 32) + n / (512 / DV));
+        }
+    }
+    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int part, int lane) const {
+        constexpr int W = DV / 64;  // pairs of values of a position
+        uint32_t pr[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float sc = scale_of(vs[i]);
+            pr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 0));
+            if constexpr (W >= 2) pr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 1));
+            if constexpr (W >= 4) {
+                pr[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 2));
+                pr[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 3));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2 * W; t++) {
+            mk_v4u o;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1][t / 2], pr[2 * i][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+            dst[part * 2 * W + t][lane] = __builtin_bit_cast(mk_b8, o);
+        }
+    }
+};
+
+// N consecutive values to the output
+template <typename T, int N> __device__ __forceinline__ void store_run(void *out, size_t at, const float (&r)[N]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *(mk_f4 *)((float *)out + at + i) = mk_f4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+    } else {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *(b4 *)((__bf16 *)out + at + i) = b4{(__bf16)r[i], (__bf16)r[i + 1], (__bf16)r[i + 2], (__bf16)r[i + 3]};
+    }
+}
+
+template <typename T, int DK, int R, int DV, int NB>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DK == 256 ? 1 : 2) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+    constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM, CT = 64 * NB;
+    __shared__ mk_b8 k_l[4][NS + NR][64], v_l[2][NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % c.nkv, split = blockIdx.x / c.nkv % a.n_splits, G = a.nh / c.nkv;
+    int b, tile;
+    if (!find_tile(s, G, CT, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    // the last position that a column of the workgroup, and that all of this wave's columns see
+    const int first = s.at(b), m_rows = max(s.at(b + 1) - first, 0), c_last = min(tile * CT + CT, m_rows * G) - 1;
+    Column col[NB];
+    int low = 0x7FFFFFFF, wtop = -1;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        col[i] = column(c, s, G, hk, b, tile * CT + (wave * NB + i) * 16 + n);
+        low = min(low, __builtin_amdgcn_readfirstlane(columns_min(col[i].live ? col[i].lim : 0x7FFFFFFF)));
+        wtop = max(wtop, __builtin_amdgcn_readfirstlane(columns_max(col[i].lim)));
+    }
+    // (limits grow with the column; a column beyond the capacity sees nothing)
+    int top = -1;
+    {
+        const int64_t lim = (int64_t)c.lens[b] - m_rows + c_last / G;
+        top = __builtin_amdgcn_readfirstlane((int)min(lim, (int64_t)c.cap - 1));
+    }
+    const int j0 = split * a.chunk, j1 = chunk_end(a, split, top + 1);
+    if (a.n_splits > 1 && j0 >= j1) return;
+
+    mk_b8 qf[NB][NS + NR][QT];
+    float m[NB], l[NB];
+    mk_f4 o[NB][NT];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        load_query<T, DK, R>(a, col[i], g, qf[i]);
+        m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[i][t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
+    const uint8_t *kqp = uniform(c.kq + row0 * (DK / 2)), *ksp = uniform(c.ks + row0 * (DK / 32)), *vqp = uniform(c.vq + row0 * (DV / 2)),
+                  *vsp = uniform(c.vs + row0 * (DV / 32)), *krp = R ? uniform(c.kr + kr0 * R) : nullptr;
+    // wave w: K of the positions 16 w .. + 15 of a step; V of the positions 32 (w / 2) .. + 31, every other tile of dimensions
+    KQuarter<DK, R> kx;
+    VQuarter<DV> vx;
+    auto fetch = [&](int j) {
+        kx.load(kqp, ksp, krp, j + 16 * wave, j1 - 1, n, g);
+        vx.load(vqp, vsp, j + 32 * (wave >> 1), j1 - 1, wave & 1, n, g);
+    };
+    if (j0 < j1) fetch(j0);
+    for (int j = j0; j < j1; j += 64) {
+        __syncthreads();
+        kx.store(k_l[wave], lane);
+        vx.store(v_l[wave >> 1], wave & 1, lane);
+        __syncthreads();
+        if (j + 64 < j1) fetch(j + 64);
+        if (j > wtop) continue;  // none of this wave's columns sees these positions
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+            float sc[NB][8];
+#pragma unroll
+            for (int ss = 0; ss < 2; ss++) {
+                mk_f4 acc[NB];
+#pragma unroll
+                for (int i = 0; i < NB; i++) acc[i] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < NS + NR; st++) {
+                    const mk_b8 kf = k_l[2 * hf + ss][st][lane];
+#pragma unroll
+                    for (int i = 0; i < NB; i++)
+#pragma unroll
+                        for (int t = 0; t < QT; t++) acc[i] = mfma(kf, qf[i][st][t], acc[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[i][4 * ss + e] = acc[i][e];
+            }
+            const int p0 = j + 32 * hf;
+            mk_b8 pf[NB][PT];
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                if (p0 + 31 > low || p0 + 32 > j1) {
+                    const int last = min(col[i].lim, j1 - 1);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (p0 + 4 * g + (e & 3) + 16 * (e >> 2) > last) sc[i][e] = -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])), fmaxf(fmaxf(sc[i][4], sc[i][5]), fmaxf(sc[i][6], sc[i][7])));
+                mx = mk_rows_max(mx);
+                if (__any(mx > m[i])) {
+                    mx = fmaxf(mx, m[i]);
+                    const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[i] - mx) * a.scale_log2);
+                    m[i] = mx;
+                    l[i] *= corr;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][t][e] *= corr;
+                }
+                const float ref = m[i] == -INFINITY ? 0.0f : m[i] * a.scale_log2;
+#pragma unroll
+                for (int e = 0; e < 8; e++) sc[i][e] = __builtin_amdgcn_exp2f(fmaf(sc[i][e], a.scale_log2, -ref));
+                l[i] += ((sc[i][0] + sc[i][1]) + (sc[i][2] + sc[i][3])) + ((sc[i][4] + sc[i][5]) + (sc[i][6] + sc[i][7]));
+                split8<PT>(sc[i], pf[i]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const mk_b8 vf = v_l[hf][t][lane];
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int k = 0; k < PT; k++) o[i][t] = mfma(vf, pf[i][k], o[i][t]);
+            }
+        }
+    }
+    float dens[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) dens[i] = mk_rows_sum(l[i]);  // (all lanes)
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        if (!col[i].live) continue;
+        const float den = dens[i];
+        const float mx = m[i] == -INFINITY ? m[i] : m[i] * a.scale_log2;
+        const size_t row = (size_t)col[i].t * a.nh + col[i].h;
+        if (a.n_splits > 1) {
+            const size_t at = (size_t)split * s.T * a.nh + row;
+            if (g == 0) a.pm[at] = mx, a.pl[at] = den;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int t = 0; t < NT; t += 4)
+                    *(mk_f4 *)(a.po + at * DV + NT * (4 * g + e) + t) = mk_f4{o[i][t][e], o[i][t + 1][e], o[i][t + 2][e], o[i][t + 3][e]};
+        } else {
+            const float inv = col[i].beyond ? __builtin_nanf("") : col[i].lim < 0 ? 0.0f : 1.0f / den;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float r[NT];
+#pragma unroll
+                for (int t = 0; t < NT; t++) r[t] = o[i][t][e] * inv;
+                store_run<T, NT>(a.out, row * DV + NT * (4 * g + e), r);
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------- the chunks' results together
 
 // One wave: (row, head).  Lane i has the statistics of chunk i: weights 2^(m_i - max), one division.
@@ -538,16 +765,29 @@ size_t column_tiles(const mk_kv4_cache *c, size_t T, const int32_t *cu, size_t g
     return cu ? T * group / ct + c->B : c->B * ((T / c->B * group + ct - 1) / ct);
 }
 
+// ct: query columns of a workgroup (16: every wave its own positions; 64, 128: the workgroup shares K and V)
+template <typename T, int D, int R>
+void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (ct == 16) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
+    else if (ct == 64) hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D, 1>), grid, dim3(256), 0, st, v, s, a);
+    else if constexpr (sizeof(T) == 2 && D < 256) hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D, 2>), grid, dim3(256), 0, st, v, s, a);
+}
 template <typename T, int D>
-void launch_few(const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
-    if (v.rope) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, 64, D>), grid, dim3(256), 0, st, v, s, a);
-    else hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, 0, D>), grid, dim3(256), 0, st, v, s, a);
+void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.rope) launch_matrix<T, D, 64>(ct, grid, st, v, s, a);
+    else launch_matrix<T, D, 0>(ct, grid, st, v, s, a);
 }
 template <typename T>
-void launch_few(const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
-    if (v.dk == 64) launch_few<T, 64>(grid, st, v, s, a);
-    else if (v.dk == 128) launch_few<T, 128>(grid, st, v, s, a);
-    else launch_few<T, 256>(grid, st, v, s, a);
+void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.dk == 64) launch_matrix<T, 64>(ct, grid, st, v, s, a);
+    else if (v.dk == 128) launch_matrix<T, 128>(ct, grid, st, v, s, a);
+    else launch_matrix<T, 256>(ct, grid, st, v, s, a);
+}
+// Query columns of a workgroup by the columns a sequence has on average: up to 16 a wave each; f32 queries (three terms) and heads of 256
+// have registers for 64, the others for 128.
+int columns_of(const mk_kv4_cache *c, int dtype, size_t T, size_t group) {
+    const size_t avg = (T * group + c->B - 1) / c->B;
+    return avg <= 16 ? 16 : avg <= 64 || dtype == MK_F32 || c->dk == 256 ? 64 : 128;
 }
 
 }  // namespace
@@ -575,7 +815,8 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
     const bool matrix = matrix_widths(c) && c->cap >= 32;
-    const size_t tiles = matrix ? column_tiles(c, T, cu, group, 16) : T * group;
+    const int ct = columns_of(c, dtype, T, group);
+    const size_t tiles = matrix ? column_tiles(c, T, cu, group, ct) : T * group;
     plan(a, tiles * c->nkv, len);
     uint8_t *w = (uint8_t *)workspace;
     a.po = (float *)w;
@@ -589,8 +830,8 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     if (matrix) {
         MK_REQUIRE(tiles * c->nkv * a.n_splits <= 0x7FFFFFFFull, "too many query rows in one call");
         const dim3 grid((unsigned)(tiles * c->nkv * a.n_splits));
-        if (dtype == MK_F32) launch_few<float>(grid, hs, v, s, a);
-        else launch_few<__bf16>(grid, hs, v, s, a);
+        if (dtype == MK_F32) launch_matrix<float>(ct, grid, hs, v, s, a);
+        else launch_matrix<__bf16>(ct, grid, hs, v, s, a);
     } else {
         const dim3 grid((unsigned)T, (unsigned)nh, (unsigned)a.n_splits);
         if (dtype == MK_F32) hipLaunchKernelGGL(kv4_attn_any_kernel<float>, grid, dim3(256), 0, hs, v, s, a);
