@@ -4,7 +4,7 @@
 namespace {
 
 constexpr int MAX_SPLITS = 64;
-constexpr int MAX_CT = 128;  // the most query columns that a workgroup of any form below takes
+constexpr int MAX_CT = 64;  // the most query columns that a workgroup of any form below takes
 
 // --------------------------------------------------------------------------------------------------- attention: any width
 
@@ -127,10 +127,11 @@ __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, At
 // f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as PT terms: three
 // for f32 results, two (17 bits) for bfloat16 results, whose own rounding is 2^-8.
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float FAR = 1048576.0f;  // 2^20: weights up to this above the reference point are summed as they are
 
 template <typename T> struct Terms;
 template <> struct Terms<float> { static constexpr int Q = 3, P = 3, PM = 3; };
-template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2, PM = 2; };
+template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2, PM = 1; };
 
 __device__ __forceinline__ mk_f4 mfma(mk_b8 a, mk_b8 b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -402,24 +403,30 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
                         if (at + 4 * g + (i & 3) + 16 * (i >> 2) >= j1) vs.vs[i] = 0;
                 }
             }
-            float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-            mx = mk_rows_max(mx);
-            if (__any(mx > m)) {
-                mx = fmaxf(mx, m);
-                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * a.scale_log2);
+            // weights against the reference point of the steps before; only where one of them is far above it (or there is none
+            // yet) is the maximum looked for and what has been summed rescaled
+            float p[8], sum;
+            auto weigh = [&](float ref) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2, -ref));
+                sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            };
+            weigh(m);
+            if (__any(!(sum < FAR))) {
+                float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+                mx = fmaxf(mk_rows_max(mx) * a.scale_log2, m);
+                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
                 m = mx;
                 l *= corr;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) o[t][i] *= corr;
+                weigh(mx == -INFINITY ? 0.0f : mx);
             }
-            const float ref = m == -INFINITY ? 0.0f : m * a.scale_log2;
-#pragma unroll
-            for (int i = 0; i < 8; i++) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2, -ref));
-            l += ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
+            l += sum;
             mk_b8 pf[PT], vt[NT];
-            split8<PT>(sc, pf);
+            split8<PT>(p, pf);
             vs.tiles(vt);
             vs.load(vqp, vsp, nat, n, g);
 #pragma unroll
@@ -433,7 +440,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
         l = mk_rows_sum(l);
     }
     // the waves' partial results: lane (n, g) holds values NT (4 g + i) + t of column n
-    if (g == 0) m_l[wave][n] = m == -INFINITY ? m : m * a.scale_log2, l_l[wave][n] = l;
+    if (g == 0) m_l[wave][n] = m, l_l[wave][n] = l;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -473,11 +480,14 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
 
 // ----------------------------------------------------------------------- many query columns: the workgroup shares K and V
 //
-// One workgroup: (tile of 64 NB query columns, kv head, chunk of the context), 64 positions a step.  Each wave turns a quarter of the
-// step's bytes into bfloat16 operands in LDS (as in the kernel above, so no transposed read is needed) and multiplies all of them
-// with its own 16 NB columns; the next step's bytes are on their way meanwhile.  A K operand read from LDS serves NB products.
-// A wave's share of a step of 64 positions: the K rows of 16 of them; the V rows of 32 of them, half of the dimensions.  Positions past
-// `last` are read as `last`.
+// One workgroup: (tile of 64 query columns, 16 a wave; kv head; chunk of the context), 32 positions a step.  Waves 0 and 1 turn the K
+// rows of 16 positions each into bfloat16 operands in LDS, waves 2 and 3 the V rows (as in the kernel above, so no transposed read
+// is needed); every wave multiplies all of them with its columns.  Software pipeline of step h, one barrier a step:
+//   scores of step h + 1 on the matrix cores, beside them the weights of step h on the vector units
+//   O += V P of step h, beside it the operands of K of step h + 2 and of V of step h + 1; the bytes of the step after are asked for
+// The statements stand in the order in which they are to be issued (sched_barrier keeps it): a matrix instruction runs for 16 cycles,
+// in which the wave can issue what does not wait for it; operands are read from LDS three products ahead.
+// A wave's share of a step: the K, or the V rows of 16 positions.  Positions past `last` are read as `last`.
 template <int DK, int R> struct KQuarter {
     static constexpr int KL = DK == 256 ? 2 : 1;
     typedef typename Raw<DK == 256 ? 16 : DK / 8>::type KT;
@@ -493,49 +503,51 @@ template <int DK, int R> struct KQuarter {
 #pragma unroll
         for (int i = 0; i < R / 32; i++) kr[i] = ldg<mk_b8>(krp, p * (R * 2) + (g * (R / 2) + 16 * i));
     }
-    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int lane) const {
-#pragma unroll
-        for (int st = 0; st < DK / 32; st++) {
+    static constexpr int SLICES = DK / 32 + R / 32;
+    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int st, int lane) const {  // operand st of the position's row
+        if (st < DK / 32) {
             uint32_t w;
             if constexpr (DK == 256) w = k[st / 4][st % 4];
             else w = k[0][st];
             dst[st][lane] = fp4x8(w, scale_of(DK == 256 ? (st < 4 ? ks & 255u : ks >> 8) : ks));
+        } else {
+            dst[st][lane] = kr[R ? st - DK / 32 : 0];
         }
-#pragma unroll
-        for (int i = 0; i < R / 32; i++) dst[DK / 32 + i][lane] = kr[i];
     }
 };
-template <> struct Raw<1> { typedef uint8_t type; };
 template <int DV> struct VQuarter {
-    typedef typename Raw<DV / 64>::type VT;
-    uint32_t v[8], vs[8];
-    __device__ __forceinline__ void load(const uint8_t *vqp, const uint8_t *vsp, int j, int last, int part, int n, int g) {
+    typedef typename Raw<DV / 32>::type VT;
+    typedef typename Raw<DV == 64 ? 4 : DV / 32>::type VL;
+    VL v[4];
+    uint32_t vs[4];
+    __device__ __forceinline__ void load(const uint8_t *vqp, const uint8_t *vsp, int j, int last, int n, int g) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t p = min(j + 4 * g + (i & 3) + 16 * (i >> 2), last);
-            v[i] = ldg<VT>(vqp, p * (DV / 2) + (n * (DV / 32) + part * (DV / 64)));
+        for (int i = 0; i < 4; i++) {
+            const uint32_t p = min(j + 4 * g + i, last);
+            v[i] = ldg<VT>(vqp, p * (DV / 2) + n * (DV / 32));
             vs[i] = ldg<uint8_t>(vsp, p * (DV / 32) + n / (512 / DV));
         }
     }
-    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int part, int lane) const {
-        constexpr int W = DV / 64;  // pairs of values of a position
-        uint32_t pr[8][4];
+    // its half (hi: positions 16 .. 31 of the 32) of the operands of the tiles 2 w and 2 w + 1
+    static constexpr int SLICES = DV / 32;
+    __device__ __forceinline__ void store(mk_b8 (*dst)[64], int w, int hi, int lane) const {
+        uint32_t pr[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 4; i++) {
             const float sc = scale_of(vs[i]);
-            pr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 0));
-            if constexpr (W >= 2) pr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 1));
-            if constexpr (W >= 4) {
-                pr[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 2));
-                pr[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], sc, 3));
-            }
+            uint32_t d;
+            if constexpr (DV == 256) d = v[i][w / 4];
+            else d = v[i];
+            const mk_b2 x = w % 4 == 0 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 0) : w % 4 == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 1)
+                          : w % 4 == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 2) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, sc, 3);
+            pr[i] = __builtin_bit_cast(uint32_t, x);
         }
 #pragma unroll
-        for (int t = 0; t < 2 * W; t++) {
-            mk_v4u o;
+        for (int t = 0; t < 2; t++) {
+            mk_u2 o;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1][t / 2], pr[2 * i][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-            dst[part * 2 * W + t][lane] = __builtin_bit_cast(mk_b8, o);
+            for (int i = 0; i < 2; i++) o[i] = __builtin_amdgcn_perm(pr[2 * i + 1], pr[2 * i], t & 1 ? 0x07060302u : 0x05040100u);
+            ((mk_u2 *)&dst[2 * w + t][lane])[hi] = o;
         }
     }
 };
@@ -552,148 +564,158 @@ template <typename T, int N> __device__ __forceinline__ void store_run(void *out
     }
 }
 
-template <typename T, int DK, int R, int DV, int NB>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DK == 256 ? 1 : 2) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
-    constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM, CT = 64 * NB;
-    __shared__ mk_b8 k_l[4][NS + NR][64], v_l[2][NT][64];
+template <typename T, int DK, int R, int DV>
+__global__ __launch_bounds__(256, DK == 256 ? 1 : sizeof(T) == 4 ? 2 : 3) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+    constexpr int NS = DK / 32, NR = R / 32, NF = NS + NR, NK = 2 * NF, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM;
+    __shared__ mk_b8 k_l[2][2][NF][64], v_l[2][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % c.nkv, split = blockIdx.x / c.nkv % a.n_splits, G = a.nh / c.nkv;
     int b, tile;
-    if (!find_tile(s, G, CT, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
+    if (!find_tile(s, G, 64, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
-    // the last position that a column of the workgroup, and that all of this wave's columns see
-    const int first = s.at(b), m_rows = max(s.at(b + 1) - first, 0), c_last = min(tile * CT + CT, m_rows * G) - 1;
-    Column col[NB];
-    int low = 0x7FFFFFFF, wtop = -1;
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        col[i] = column(c, s, G, hk, b, tile * CT + (wave * NB + i) * 16 + n);
-        low = min(low, __builtin_amdgcn_readfirstlane(columns_min(col[i].live ? col[i].lim : 0x7FFFFFFF)));
-        wtop = max(wtop, __builtin_amdgcn_readfirstlane(columns_max(col[i].lim)));
-    }
-    // (limits grow with the column; a column beyond the capacity sees nothing)
-    int top = -1;
-    {
-        const int64_t lim = (int64_t)c.lens[b] - m_rows + c_last / G;
-        top = __builtin_amdgcn_readfirstlane((int)min(lim, (int64_t)c.cap - 1));
-    }
+    const Column col = column(c, s, G, hk, b, tile * 64 + wave * 16 + n);
+    const int low = __builtin_amdgcn_readfirstlane(columns_min(col.live ? col.lim : 0x7FFFFFFF));
+    // the last position that a column of the workgroup sees (limits grow with the column; one beyond the capacity sees nothing)
+    const int first = s.at(b), m_rows = max(s.at(b + 1) - first, 0), c_last = min(tile * 64 + 64, m_rows * G) - 1;
+    const int top = __builtin_amdgcn_readfirstlane((int)min((int64_t)c.lens[b] - m_rows + c_last / G, (int64_t)c.cap - 1));
     const int j0 = split * a.chunk, j1 = chunk_end(a, split, top + 1);
     if (a.n_splits > 1 && j0 >= j1) return;
 
-    mk_b8 qf[NB][NS + NR][QT];
-    float m[NB], l[NB];
-    mk_f4 o[NB][NT];
+    mk_b8 qf[NF][QT];
+    load_query<T, DK, R>(a, col, g, qf);
+    float m = -INFINITY, l = 0.0f;
+    mk_f4 o[NT];
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-        load_query<T, DK, R>(a, col[i], g, qf[i]);
-        m[i] = -INFINITY, l[i] = 0.0f;
+    for (int t = 0; t < NT; t++) o[t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (j0 < j1) {
+        const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
+        const uint8_t *kqp = uniform(c.kq + row0 * (DK / 2)), *ksp = uniform(c.ks + row0 * (DK / 32)), *vqp = uniform(c.vq + row0 * (DV / 2)),
+                      *vsp = uniform(c.vs + row0 * (DV / 32)), *krp = R ? uniform(c.kr + kr0 * R) : nullptr;
+        const bool k_wave = wave < 2;
+        const int half = wave & 1;
+        KQuarter<DK, R> kx;
+        VQuarter<DV> vx;
+        auto fetch_k = [&](int j) { kx.load(kqp, ksp, krp, j + 16 * half, j1 - 1, n, g); };
+        auto fetch_v = [&](int j) { vx.load(vqp, vsp, j + 16 * half, j1 - 1, n, g); };
+        auto store_k = [&](int buf) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) o[i][t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const size_t row0 = ((size_t)b * c.nkv + hk) * c.cap, kr0 = (size_t)b * c.cap;
-    const uint8_t *kqp = uniform(c.kq + row0 * (DK / 2)), *ksp = uniform(c.ks + row0 * (DK / 32)), *vqp = uniform(c.vq + row0 * (DV / 2)),
-                  *vsp = uniform(c.vs + row0 * (DV / 32)), *krp = R ? uniform(c.kr + kr0 * R) : nullptr;
-    // wave w: K of the positions 16 w .. + 15 of a step; V of the positions 32 (w / 2) .. + 31, every other tile of dimensions
-    KQuarter<DK, R> kx;
-    VQuarter<DV> vx;
-    auto fetch = [&](int j) {
-        kx.load(kqp, ksp, krp, j + 16 * wave, j1 - 1, n, g);
-        vx.load(vqp, vsp, j + 32 * (wave >> 1), j1 - 1, wave & 1, n, g);
-    };
-    if (j0 < j1) fetch(j0);
-    for (int j = j0; j < j1; j += 64) {
-        __syncthreads();
-        kx.store(k_l[wave], lane);
-        vx.store(v_l[wave >> 1], wave & 1, lane);
-        __syncthreads();
-        if (j + 64 < j1) fetch(j + 64);
-        if (j > wtop) continue;  // none of this wave's columns sees these positions
+            for (int i = 0; i < NF; i++) kx.store(k_l[buf][half], i, lane);
+        };
+        mk_f4 sc[2], nx[2];  // scores of this step and of the next
+        if (k_wave) {
+            fetch_k(j0);
+            store_k(0);
+            fetch_k(j0 + 32);
+            store_k(1);
+            fetch_k(j0 + 64);
+        } else {
+            fetch_v(j0);
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            float sc[NB][8];
+            for (int i = 0; i < NT / 2; i++) vx.store(v_l[0], i, half, lane);
+            fetch_v(j0 + 32);
+        }
+        mk_wg_barrier();
 #pragma unroll
-            for (int ss = 0; ss < 2; ss++) {
-                mk_f4 acc[NB];
+        for (int k = 0; k < NK; k++) {
+            const mk_b8 kf = k_l[0][k / NF][k % NF][lane];
 #pragma unroll
-                for (int i = 0; i < NB; i++) acc[i] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < QT; t++) sc[k / NF] = mfma(kf, qf[k % NF][t], k % NF || t ? sc[k / NF] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
+        mk_wg_barrier();  // (the first step stores into K's first buffer)
+        for (int j = j0, buf = 0; j < j1; j += 32, buf ^= 1) {
+            if (j + 31 > low || j + 32 > j1) {
+                const int last = min(col.lim, j1 - 1) - j - 4 * g;
 #pragma unroll
-                for (int st = 0; st < NS + NR; st++) {
-                    const mk_b8 kf = k_l[2 * hf + ss][st][lane];
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int i = 0; i < NB; i++)
-#pragma unroll
-                        for (int t = 0; t < QT; t++) acc[i] = mfma(kf, qf[i][st][t], acc[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < NB; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sc[i][4 * ss + e] = acc[i][e];
+                    for (int e = 0; e < 4; e++)
+                        if (16 * u + e > last) sc[u][e] = -INFINITY;
             }
-            const int p0 = j + 32 * hf;
-            mk_b8 pf[NB][PT];
+            float p[8], sum;
+            const mk_b8 (*kn)[NF][64] = k_l[buf ^ 1];
+            mk_b8 ring[4];
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
-                if (p0 + 31 > low || p0 + 32 > j1) {
-                    const int last = min(col[i].lim, j1 - 1);
+            for (int k = 0; k < 3; k++) ring[k] = kn[k / NF][k % NF][lane];
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (p0 + 4 * g + (e & 3) + 16 * (e >> 2) > last) sc[i][e] = -INFINITY;
-                }
-                float mx = fmaxf(fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])), fmaxf(fmaxf(sc[i][4], sc[i][5]), fmaxf(sc[i][6], sc[i][7])));
-                mx = mk_rows_max(mx);
-                if (__any(mx > m[i])) {
-                    mx = fmaxf(mx, m[i]);
-                    const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[i] - mx) * a.scale_log2);
-                    m[i] = mx;
-                    l[i] *= corr;
+            for (int k = 0; k < NK; k++) {
+                const int u = k / NF, st = k % NF;
+                if (k + 3 < NK) ring[(k + 3) & 3] = kn[(k + 3) / NF][(k + 3) % NF][lane];
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                for (int t = 0; t < QT; t++) nx[u] = mfma(ring[k & 3], qf[st][t], st || t ? nx[u] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[i][t][e] *= corr;
-                }
-                const float ref = m[i] == -INFINITY ? 0.0f : m[i] * a.scale_log2;
-#pragma unroll
-                for (int e = 0; e < 8; e++) sc[i][e] = __builtin_amdgcn_exp2f(fmaf(sc[i][e], a.scale_log2, -ref));
-                l[i] += ((sc[i][0] + sc[i][1]) + (sc[i][2] + sc[i][3])) + ((sc[i][4] + sc[i][5]) + (sc[i][6] + sc[i][7]));
-                split8<PT>(sc[i], pf[i]);
+                for (int e = 8 * k / NK; e < 8 * (k + 1) / NK; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][e % 4], a.scale_log2, -m));
+                __builtin_amdgcn_sched_barrier(0);
             }
+            auto add = [&]() { sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])); };
+            add();
+            // only where a weight is far above the reference point of the steps before (or there is none yet) is the maximum looked
+            // for and what has been summed rescaled
+            if (__any(!(sum < FAR))) {
+                float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+                mx = fmaxf(mk_rows_max(mx) * a.scale_log2, m);
+                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx), ref = mx == -INFINITY ? 0.0f : mx;
+                m = mx;
+                l *= corr;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const mk_b8 vf = v_l[hf][t][lane];
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int i = 0; i < NB; i++)
+                    for (int e = 0; e < 4; e++) o[t][e] *= corr;
 #pragma unroll
-                    for (int k = 0; k < PT; k++) o[i][t] = mfma(vf, pf[i][k], o[i][t]);
+                for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], a.scale_log2, -ref));
+                add();
             }
+            l += sum;
+#pragma unroll
+            for (int k = 0; k < 3; k++) ring[k] = v_l[buf][k][lane];
+            mk_b8 pf[PT];
+            split8<PT>(p, pf);
+            __builtin_amdgcn_sched_barrier(0);
+            auto out_tile = [&](int t) {
+                if (t + 3 < NT) ring[(t + 3) & 3] = v_l[buf][t + 3][lane];
+#pragma unroll
+                for (int k = 0; k < PT; k++) o[t] = mfma(ring[t & 3], pf[k], o[t]);
+            };
+            if (k_wave) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    out_tile(t);
+#pragma unroll
+                    for (int e = NF * t / NT; e < NF * (t + 1) / NT; e++) kx.store(k_l[buf][half], e, lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                fetch_k(j + 96);
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    out_tile(t);
+                    if (t % 2 == 0) vx.store(v_l[buf ^ 1], t / 2, half, lane);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                fetch_v(j + 64);
+            }
+            sc[0] = nx[0], sc[1] = nx[1];
+            mk_wg_barrier();
         }
     }
-    float dens[NB];
+    const float den = mk_rows_sum(l);
+    if (!col.live) return;
+    const size_t row = (size_t)col.t * a.nh + col.h;
+    if (a.n_splits > 1) {
+        const size_t at = (size_t)split * s.T * a.nh + row;
+        if (g == 0) a.pm[at] = m, a.pl[at] = den;
 #pragma unroll
-    for (int i = 0; i < NB; i++) dens[i] = mk_rows_sum(l[i]);  // (all lanes)
+        for (int e = 0; e < 4; e++)
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-        if (!col[i].live) continue;
-        const float den = dens[i];
-        const float mx = m[i] == -INFINITY ? m[i] : m[i] * a.scale_log2;
-        const size_t row = (size_t)col[i].t * a.nh + col[i].h;
-        if (a.n_splits > 1) {
-            const size_t at = (size_t)split * s.T * a.nh + row;
-            if (g == 0) a.pm[at] = mx, a.pl[at] = den;
+            for (int t = 0; t < NT; t += 4) *(mk_f4 *)(a.po + at * DV + NT * (4 * g + e) + t) = mk_f4{o[t][e], o[t + 1][e], o[t + 2][e], o[t + 3][e]};
+    } else {
+        const float inv = col.beyond ? __builtin_nanf("") : col.lim < 0 ? 0.0f : 1.0f / den;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+        for (int e = 0; e < 4; e++) {
+            float r[NT];
 #pragma unroll
-                for (int t = 0; t < NT; t += 4)
-                    *(mk_f4 *)(a.po + at * DV + NT * (4 * g + e) + t) = mk_f4{o[i][t][e], o[i][t + 1][e], o[i][t + 2][e], o[i][t + 3][e]};
-        } else {
-            const float inv = col[i].beyond ? __builtin_nanf("") : col[i].lim < 0 ? 0.0f : 1.0f / den;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float r[NT];
-#pragma unroll
-                for (int t = 0; t < NT; t++) r[t] = o[i][t][e] * inv;
-                store_run<T, NT>(a.out, row * DV + NT * (4 * g + e), r);
-            }
+            for (int t = 0; t < NT; t++) r[t] = o[t][e] * inv;
+            store_run<T, NT>(a.out, row * DV + NT * (4 * g + e), r);
         }
     }
 }
@@ -738,11 +760,14 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnA
 // 256 positions (two steps a wave) a chunk is start and end only, above 1024 one long sequence among short ones is a tail (32
 // ragged sequences: 38.6 / 35.4 / 41.1 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
 // costs what the split saves (96 heads, 1024 positions: 13.2 us, in four chunks 10.3 + 4.0 us).
-void plan(AttnArgs &a, size_t pairs, size_t len) {
-    size_t chunk = (pairs * len / 1024 + 127) / 128 * 128;
-    chunk = len <= 1024 ? len : chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+// Many columns: a chunk's result is as large as its columns and the work is bound by the matrix cores, so a context is cut only while
+// the workgroups are fewer than the compute units (512 rows at 4096 positions, 96 heads: four chunks and their merge cost 32 us).
+void plan(AttnArgs &a, size_t pairs, size_t len, int ct) {
+    size_t chunk = (pairs * len / (ct > 16 ? 512 : 1024) + 127) / 128 * 128;
+    if (ct > 16) chunk = len <= 1024 || pairs >= 256 ? len : chunk < 256 ? 256 : chunk;
+    else chunk = len <= 1024 ? len : chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
     const size_t least = (len + MAX_SPLITS - 1) / MAX_SPLITS;
-    if (chunk < least) chunk = (least + 127) / 128 * 128;
+    if (chunk < least && chunk < len) chunk = (least + 127) / 128 * 128;
     a.chunk = (int)chunk;
     a.n_splits = (int)((len + chunk - 1) / chunk);
 }
@@ -765,12 +790,11 @@ size_t column_tiles(const mk_kv4_cache *c, size_t T, const int32_t *cu, size_t g
     return cu ? T * group / ct + c->B : c->B * ((T / c->B * group + ct - 1) / ct);
 }
 
-// ct: query columns of a workgroup (16: every wave its own positions; 64, 128: the workgroup shares K and V)
+// ct: query columns of a workgroup (16: every wave its own positions; 64: the workgroup shares K and V)
 template <typename T, int D, int R>
 void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
     if (ct == 16) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
-    else if (ct == 64) hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D, 1>), grid, dim3(256), 0, st, v, s, a);
-    else if constexpr (sizeof(T) == 2 && D < 256) hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D, 2>), grid, dim3(256), 0, st, v, s, a);
+    else hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
 }
 template <typename T, int D>
 void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
@@ -783,12 +807,8 @@ void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, con
     else if (v.dk == 128) launch_matrix<T, 128>(ct, grid, st, v, s, a);
     else launch_matrix<T, 256>(ct, grid, st, v, s, a);
 }
-// Query columns of a workgroup by the columns a sequence has on average: up to 16 a wave each; f32 queries (three terms) and heads of 256
-// have registers for 64, the others for 128.
-int columns_of(const mk_kv4_cache *c, int dtype, size_t T, size_t group) {
-    const size_t avg = (T * group + c->B - 1) / c->B;
-    return avg <= 16 ? 16 : avg <= 64 || dtype == MK_F32 || c->dk == 256 ? 64 : 128;
-}
+// Query columns of a workgroup, by the columns a sequence has on average: a wave's 16 are all there is, or the workgroup shares K and V.
+int columns_of(const mk_kv4_cache *c, size_t T, size_t group) { return T * group <= 16 * c->B ? 16 : 64; }
 
 }  // namespace
 
@@ -815,9 +835,9 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
     const bool matrix = matrix_widths(c) && c->cap >= 32;
-    const int ct = columns_of(c, dtype, T, group);
+    const int ct = columns_of(c, T, group);
     const size_t tiles = matrix ? column_tiles(c, T, cu, group, ct) : T * group;
-    plan(a, tiles * c->nkv, len);
+    plan(a, tiles * c->nkv, len, matrix ? ct : 16);
     uint8_t *w = (uint8_t *)workspace;
     a.po = (float *)w;
     w += mk_align_up((size_t)a.n_splits * T * nh * c->dv * 4, 256);

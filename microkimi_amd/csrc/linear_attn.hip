@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
     double total = 0.0;
     if (threadIdx.x == 0) bad_l = 0;
     for (int c = c0; c < c1; c++) {
-        __syncthreads();
+        mk_wg_barrier();
         bool ok = true;
 #pragma unroll
         for (int i = 0; i < KP; i++) {
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
             if (lane == 0) last_l = expf((float)end);
             total += end;
         }
-        __syncthreads();
+        mk_wg_barrier();
         if (c + 1 < c1) fetch(c + 1);
         if constexpr (OUT) {
             // scores of the wave's 16 query tokens
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
                 }
                 p_l[s2 == 0 ? wave : 2 + wave][lane] = operand<T>(pt[0], pt[1]);  // (second half: queries 32 .. 63 only)
             }
-            __syncthreads();
+            mk_wg_barrier();
         }
         F vt[NT][2];
 #pragma unroll

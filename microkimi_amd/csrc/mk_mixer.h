@@ -8,6 +8,10 @@ typedef __bf16 mk_b2 __attribute__((ext_vector_type(2)));
 static inline size_t mk_align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 static inline bool mk_aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+// Workgroup barrier that waits for this wave's LDS traffic only: __syncthreads() waits for the global loads in flight too, which would put
+// the latency of the next step's prefetch into every barrier.
+__device__ __forceinline__ void mk_wg_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <typename T> __device__ __forceinline__ void mk_load8(const T *p, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
         const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 4);
