@@ -636,11 +636,11 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : sizeof(T) == 4 ? 2 : 3) void k
             const mk_b8 (*kn)[NF][64] = k_l[buf ^ 1];
             mk_b8 ring[4];
 #pragma unroll
-            for (int k = 0; k < 3; k++) ring[k] = kn[k / NF][k % NF][lane];
+            for (int k = 0; k < 3; k++) ring[k] = kn[k % 2][k / 2][lane];
 #pragma unroll
             for (int k = 0; k < NK; k++) {
-                const int u = k / NF, st = k % NF;
-                if (k + 3 < NK) ring[(k + 3) & 3] = kn[(k + 3) / NF][(k + 3) % NF][lane];
+                const int u = k % 2, st = k / 2;  // two sums in turn: one waits for itself longer than an instruction runs
+                if (k + 3 < NK) ring[(k + 3) & 3] = kn[(k + 3) % 2][(k + 3) / 2][lane];
 #pragma unroll
                 for (int t = 0; t < QT; t++) nx[u] = mfma(ring[k & 3], qf[st][t], st || t ? nx[u] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
