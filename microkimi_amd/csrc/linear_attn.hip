@@ -195,6 +195,8 @@ template <int LD, int RUN> __device__ __forceinline__ mk_f8v column8(const float
     return f;
 }
 
+template <int N> struct Int { static constexpr int value = N; };
+
 struct LinSeg {
     int n_seg;
     mk_f4 *local;   // [b][h][segment][DK / 16 * NT][256]: local states, then the states before each segment
@@ -208,6 +210,9 @@ __device__ __forceinline__ void segment(int n, int n_seg, int seg, int &c0, int 
 }
 // dv column of (lane, tile t) within the state: a wave's quarter, 8 consecutive values in the two tiles of a lane group
 template <int NT> __device__ __forceinline__ int state_col(int wave, int n, int t) { return NT == 2 ? 32 * wave + 8 * (n >> 2) + 4 * t + (n & 3) : 16 * wave + n; }
+
+// 2^x for the decays: x is a difference of 64-bit sums of log2 decays, rounded once
+__device__ __forceinline__ float pow2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
 // inclusive sum over the wave in 64 bits
 __device__ __forceinline__ double wave_scan(double v, int lane) {
@@ -226,8 +231,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / 256, VP = CH * DV / E / 256;  // values of a 16-byte piece; pieces a thread moves
     __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LK : 8];
     __shared__ F p_l[OUT ? 6 : 1][64];
-    __shared__ double b_l[CH];
-    __shared__ float w_l[CH], e_l[CH], last_l;
+    __shared__ double b_l[2][CH];                       // sums of the log2 decays of a block and of the next
+    __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
     __shared__ int bad_l;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int h = blockIdx.x % a.nh, seg = blockIdx.x / a.nh % sg.n_seg, b = blockIdx.x / a.nh / sg.n_seg, hk = h / (a.nh / a.nkh);
@@ -253,83 +258,97 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
     const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * DV;
     mk_v4u kr[KP], vr[VP], qr[OUT ? KP : 1];
     float gr;
-    auto fetch = [&](int c) {  // the block's rows into registers; behind the sequence: zeros, and no decay
-        const int first = c * CH;
+    // A block's rows into registers: a scalar base, a lane offset that never changes, and a scalar step from piece to piece.  Rows behind the
+    // sequence are read as its last one (and dropped at the store).
+    const int rk = threadIdx.x / (DK / E), rv = threadIdx.x / (DV / E), dk0 = threadIdx.x % (DK / E) * E, dv0 = threadIdx.x % (DV / E) * E;
+    auto rows = [&](mk_v4u *dst, const T *base, size_t stride, int first, int r0, int d0, auto pieces, auto step) {
+        const T *p = base + (size_t)(t0 + first) * stride;
+        if (first + CH <= len) {
+            const uint32_t off = (uint32_t)(r0 * (uint32_t)stride + d0) * sizeof(T);
 #pragma unroll
-        for (int i = 0; i < KP; i++) {
-            const int at = i * 256 + threadIdx.x, r = first + at / (DK / E), d = at % (DK / E) * E;
-            const size_t row = (size_t)(t0 + min(r, len - 1));
-            const bool in = r < len;
-            const mk_v4u x = *(const mk_v4u *)(kp + row * a.ks + d);
-            kr[i] = in ? x : mk_v4u{0, 0, 0, 0};
-            if constexpr (OUT) {
-                const mk_v4u y = *(const mk_v4u *)(qp + row * a.qs + d);
-                qr[i] = in ? y : mk_v4u{0, 0, 0, 0};
-            }
-        }
+            for (int i = 0; i < decltype(pieces)::value; i++) dst[i] = *(const MK_GLOBAL mk_v4u *)((const MK_GLOBAL uint8_t *)(p + i * (decltype(step)::value * stride)) + off);
+        } else {
 #pragma unroll
-        for (int i = 0; i < VP; i++) {
-            const int at = i * 256 + threadIdx.x, r = first + at / (DV / E), d = at % (DV / E) * E;
-            const mk_v4u x = *(const mk_v4u *)(vp + (size_t)(t0 + min(r, len - 1)) * a.vs + d);
-            vr[i] = r < len ? x : mk_v4u{0, 0, 0, 0};
+            for (int i = 0; i < decltype(pieces)::value; i++) dst[i] = *(const mk_v4u *)(p + (size_t)min(r0 + i * decltype(step)::value, len - 1 - first) * stride + d0);
         }
-        const float x = a.g[a.gs ? (size_t)(t0 + min(first + lane, len - 1)) * a.gs + h : h];
-        gr = first + lane < len ? (x < -200.0f ? -200.0f : x) : 0.0f;
     };
-    if (c0 < c1) fetch(c0);
+    auto fetch = [&](int c) {
+        rows(kr, kp, a.ks, c * CH, rk, dk0, Int<KP>(), Int<CH / KP>());
+        if constexpr (OUT) rows(qr, qp, a.qs, c * CH, rk, dk0, Int<KP>(), Int<CH / KP>());
+        rows(vr, vp, a.vs, c * CH, rv, dv0, Int<VP>(), Int<CH / VP>());
+    };
+    auto decays = [&](int c) { return a.g[a.gs ? (size_t)(t0 + min(c * CH + lane, len - 1)) * a.gs + h : h]; };
     double total = 0.0;
+    auto scan = [&](int c, float gr) {  // one wave: the sums of block c
+        const int u = c & 1;
+        const double s = wave_scan(c * CH + lane < len ? (double)(gr < -200.0f ? -200.0f : gr) * 1.4426950408889634 : 0.0, lane), end = __shfl(s, 63, MK_WAVE);
+        b_l[u][lane] = s;
+        w_l[u][lane] = pow2(end - s);
+        e_l[u][lane] = pow2(s) * a.scale;
+        if (lane == 0) last_l[u] = pow2(end);
+        total += end;
+    };
+    if (c0 < c1) {
+        fetch(c0);
+        if (wave == 0) {
+            scan(c0, decays(c0));
+            gr = decays(c0 + 1);
+        }
+    }
     if (threadIdx.x == 0) bad_l = 0;
     for (int c = c0; c < c1; c++) {
         mk_wg_barrier();
         bool ok = true;
+        const int left = len - c * CH;  // tokens from this block on: behind them zeros, and no decay
+        const mk_v4u zero = mk_v4u{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < KP; i++) {
             const int at = i * 256 + threadIdx.x, r = at / (DK / E), d = at % (DK / E) * E;
-            *(mk_v4u *)&k_l[r * LK + d] = kr[i];
-            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + d] = qr[i];
+            *(mk_v4u *)&k_l[r * LK + d] = r < left ? kr[i] : zero;
+            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + d] = r < left ? qr[i] : zero;
         }
 #pragma unroll
         for (int i = 0; i < VP; i++) {
             const int at = i * 256 + threadIdx.x, r = at / (DV / E), d = at % (DV / E) * E;
-            *(mk_v4u *)&v_l[r * LV + d] = vr[i];
-            ok &= Op<T>::finite(vr[i]);
+            const mk_v4u x = r < left ? vr[i] : zero;
+            *(mk_v4u *)&v_l[r * LV + d] = x;
+            ok &= Op<T>::finite(x);
         }
         if (OUT && !ok) bad_l = c + 1;
-        if (wave == 0) {
-            const double s = wave_scan((double)gr, lane), end = __shfl(s, 63, MK_WAVE);
-            b_l[lane] = s;
-            w_l[lane] = expf((float)(end - s));
-            e_l[lane] = expf((float)s);
-            if (lane == 0) last_l = expf((float)end);
-            total += end;
-        }
         mk_wg_barrier();
         if (c + 1 < c1) fetch(c + 1);
+        const int u = c & 1;
         if constexpr (OUT) {
             // scores of the wave's 16 query tokens
             F qf[DK / 32];
 #pragma unroll
             for (int s = 0; s < DK / 32; s++) qf[s] = row8(&q_l[(16 * wave + n) * LK + 32 * s + 8 * g]);
-            const double bq = b_l[16 * wave + n];
+            const double bq = b_l[u][16 * wave + n];
             for (int s2 = 0; s2 <= wave / 2; s2++) {
                 mk_f4 pt[2];
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int i = 2 * s2 + u;
-                    pt[u] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int v = 0; v < 2; v++) {
+                    const int i = 2 * s2 + v;
+                    pt[v] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
                     if (i <= wave) {
 #pragma unroll
-                        for (int s = 0; s < DK / 32; s++) pt[u] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[u]);
+                        for (int s = 0; s < DK / 32; s++) pt[v] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[v]);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int key = 16 * i + 4 * g + j;
-                            pt[u][j] = key <= 16 * wave + n ? pt[u][j] * expf((float)(bq - b_l[key])) : 0.0f;
+                        for (int j = 0; j < 4; j++) pt[v][j] *= pow2(bq - b_l[u][16 * i + 4 * g + j]) * a.scale;
+                        if (i == wave) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                if (4 * g + j > n) pt[v][j] = 0.0f;
                         }
                     }
                 }
                 p_l[s2 == 0 ? wave : 2 + wave][lane] = operand<T>(pt[0], pt[1]);  // (second half: queries 32 .. 63 only)
             }
+            // (the wave with the fewest scores forms the next block's sums)
+            if (wave == 0 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
             mk_wg_barrier();
+        } else {
+            if (wave == 0 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
         }
         F vt[NT][2];
 #pragma unroll
@@ -349,7 +368,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
 #pragma unroll
                 for (int s = 0; s < DK / 32; s++) qb[s] = row44(&q_l[(16 * j + n) * LK + 32 * s + 4 * g]);
                 mk_f4 o[NT];
-                const float e = e_l[16 * j + n];
+                const float e = e_l[u][16 * j + n];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     o[t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -379,19 +398,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
                 if (tok < len) {
                     T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + state_col<NT>(wave, 4 * g, 0);
                     if constexpr (NT == 2) {
-                        const mk_f4 lo = o[0] * a.scale, hi = o[1] * a.scale;
+                        const mk_f4 lo = o[0], hi = o[1];
                         if constexpr (sizeof(T) == 4) *(mk_f4 *)dst = lo, *(mk_f4 *)(dst + 4) = hi;
                         else *(mk_b8 *)dst = operand<T>(lo, hi);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) dst[i] = (T)(o[0][i] * a.scale);
+                        for (int i = 0; i < 4; i++) dst[i] = (T)o[0][i];
                     }
                 }
             }
         }
         // the state behind the block
         if (!OUT || sg.n_seg == 1 || c + 1 < c1) {
-            const float end = last_l;
+            const float end = last_l[u];
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
@@ -402,8 +421,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
             for (int ks = 0; ks < 2; ks++) {
                 F wv[NT][Op<T>::TERMS];
                 float w[8];
-                *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[32 * ks + 4 * g];
-                *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[32 * ks + 16 + 4 * g];
+                *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[u][32 * ks + 4 * g];
+                *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[u][32 * ks + 16 + 4 * g];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     float r[8];
@@ -440,7 +459,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
                 mine[(kt * NT + t) * 256] = S[kt][t];
             }
         }
-    if (!OUT && threadIdx.x == 0) sg.decay[bh * sg.n_seg + seg] = expf((float)total);
+    if (!OUT && threadIdx.x == 0) sg.decay[bh * sg.n_seg + seg] = pow2(total);
 }
 
 // Between the two passes over the segments: local states -> the states before each segment, and the state behind the last.  One
@@ -521,6 +540,7 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
     MK_REQUIRE(dk >= 8 && dk <= 256 && dk % 8 == 0 && dv >= 8 && dv <= 256 && dv % 8 == 0, "head widths must be multiples of 8 up to 256");
     MK_REQUIRE(g && state_out && (T == 0 || (q && k && v && out)), "null pointer");
     MK_REQUIRE(qs % 8 == 0 && ks % 8 == 0 && vs % 8 == 0, "token strides must be multiples of 8 values");
+    MK_REQUIRE(qs <= 0x7FFFFF && ks <= 0x7FFFFF && vs <= 0x7FFFFF, "a token stride is out of range");
     MK_REQUIRE(T <= 1 || (qs >= nkh * dk && ks >= nkh * dk && vs >= nh * dv && (gs == 0 || gs >= nh)), "a token stride is shorter than a token's heads");
     MK_REQUIRE(mk_aligned16(q) && mk_aligned16(k) && mk_aligned16(v) && mk_aligned16(out) && mk_aligned16(state) && mk_aligned16(state_out), "pointers must be 16-byte aligned");
     return MK_OK;
