@@ -113,12 +113,11 @@ int launch_token(const LinArgs &a, hipStream_t st) {
 // which is all matrix products, and every exponent of the decays is a difference of sums of the same block: formed in 64 bits, so that
 // no large sum cancels, it is never positive for log decays that are not (a log decay below -200 counts as -200: e^-200 is 0).
 //
-// One workgroup: a run of blocks of (value head, sequence), its four waves a quarter of dv each.  The state stays in registers
-// across the blocks, as the matrix instruction returns it: tile (kt, t) of S = rows 16 kt + 4 g + j, column n (lane = 16 g + n).  Two
-// such tiles ARE an operand of the next product once the sum over dk takes its terms in the order {4 g .. , 16 + 4 g ..}; the same
-// holds for the block's scores and the sum over its tokens.  So the waves exchange only the scores (each computes those of 16
-// query tokens), through LDS in operand order.
-//   scores   A = K rows, B = Q rows               -> (key, query), weighted by the decay, masked, to LDS
+// One workgroup: a run of blocks of (value head, sequence), one wave for every 16 columns of dv.  The state stays in registers across the
+// blocks, as the matrix instruction returns it: tile kt of S = rows 16 kt + 4 g + j, the wave's column n (lane = 16 g + n).  Two such
+// tiles ARE an operand of the next product once the sum over dk takes its terms in the order {4 g .. , 16 + 4 g ..}; the same
+// holds for the block's scores and the sum over its tokens.  So the waves exchange only the scores, through LDS in operand order:
+//   scores   A = K rows, B = Q rows               -> (key, query), weighted by the decay, masked, to LDS (six operands, shared out)
 //   out      A = S^T, B = Q^T; times e^{b_i}; A = V^T, B = scores     -> (dv, token)
 //   state    A = K^T, B = weighted V^T            -> (dk, dv)
 // bfloat16 rows: S and the weighted scores are rounded to bfloat16 for the products of the output (whose own rounding is as large);
@@ -177,19 +176,18 @@ __device__ __forceinline__ mk_f8v row44(const float *p) {
     const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 16);
     return mk_f8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-// a transposed operand of a tile in LDS [token][LD]: lane (g, n) gets column col(n) of the tokens 32 ks + 4 g .. + 3 and 16 further; the
-// columns of the 16 lanes of a group are four runs of four, run r at cols + RUN * r
-template <int LD, int RUN> __device__ __forceinline__ mk_b8 column8(const __bf16 *tile, int ks, int cols, int g, int n) {
+// a transposed operand of a tile in LDS [token][LD]: lane (g, n) gets column cols + n of the tokens 32 ks + 4 g .. + 3 and 16 further
+template <int LD> __device__ __forceinline__ mk_b8 column8(const __bf16 *tile, int ks, int cols, int g, int n) {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    const __bf16 *p = tile + (32 * ks + 4 * g + (n >> 2)) * LD + cols + RUN * (n & 3);
+    const __bf16 *p = tile + (32 * ks + 4 * g + (n >> 2)) * LD + cols + 4 * (n & 3);
     const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p);
     const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p + 16 * LD));
     typedef short s8 __attribute__((ext_vector_type(8)));
     return __builtin_bit_cast(mk_b8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
-template <int LD, int RUN> __device__ __forceinline__ mk_f8v column8(const float *tile, int ks, int cols, int g, int n) {
+template <int LD> __device__ __forceinline__ mk_f8v column8(const float *tile, int ks, int cols, int g, int n) {
     mk_f8v f;
-    const float *p = tile + (32 * ks + 4 * g) * LD + cols + RUN * (n >> 2) + (n & 3);
+    const float *p = tile + (32 * ks + 4 * g) * LD + cols + n;
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = p[((i & 3) + 16 * (i >> 2)) * LD];
     return f;
@@ -199,7 +197,7 @@ template <int N> struct Int { static constexpr int value = N; };
 
 struct LinSeg {
     int n_seg;
-    mk_f4 *local;   // [b][h][segment][DK / 16 * NT][256]: local states, then the states before each segment
+    mk_f4 *local;   // [b][h][segment][DK / 16][threads]: local states, then the states before each segment
     float *decay;   // [b][h][segment]: e^{sum of the segment's log decays}
 };
 // blocks of segment seg of a sequence with n tokens
@@ -208,9 +206,6 @@ __device__ __forceinline__ void segment(int n, int n_seg, int seg, int &c0, int 
     c0 = min(seg * per, nch);
     c1 = min(c0 + per, nch);
 }
-// dv column of (lane, tile t) within the state: a wave's quarter, 8 consecutive values in the two tiles of a lane group
-template <int NT> __device__ __forceinline__ int state_col(int wave, int n, int t) { return NT == 2 ? 32 * wave + 8 * (n >> 2) + 4 * t + (n & 3) : 16 * wave + n; }
-
 // 2^x for the decays: x is a difference of 64-bit sums of log2 decays, rounded once
 __device__ __forceinline__ float pow2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
@@ -225,12 +220,12 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
 }
 
 template <typename T, int DK, int DV, bool OUT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kernel(LinArgs a, LinSeg sg) {
+__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) : (OUT && DK > DV ? 1 : 2)) void linear_block_kernel(LinArgs a, LinSeg sg) {
     typedef typename Op<T>::F F;
-    constexpr int NT = DV / 64, KT = DK / 16, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, RUN = NT == 2 ? 8 : 4;
-    constexpr int E = 16 / sizeof(T), KP = CH * DK / E / 256, VP = CH * DV / E / 256;  // values of a 16-byte piece; pieces a thread moves
+    constexpr int NW = DV / 16, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD;
+    constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
     __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LK : 8];
-    __shared__ F p_l[OUT ? 6 : 1][64];
+    __shared__ F p_l[OUT ? 6 : 1][64];                  // scores: query tiles 0 .. 3 with keys 0 .. 31, query tiles 2, 3 with keys 32 .. 63
     __shared__ double b_l[2][CH];                       // sums of the log2 decays of a block and of the next
     __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
     __shared__ int bad_l;
@@ -239,28 +234,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
     const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0);
     int c0, c1;
     segment(len, sg.n_seg, seg, c0, c1);
-    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV;
+    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV + 16 * wave + n;
     if (c0 >= c1 && sg.n_seg > 1) return;
-    mk_f4 S[KT][NT];
-    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT * NT) * 256 + threadIdx.x;
+    mk_f4 S[KT];
+    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT) * TH + threadIdx.x;
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++)
+    for (int kt = 0; kt < KT; kt++) {
+        S[kt] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (OUT && sg.n_seg > 1) {
+            S[kt] = mine[kt * TH];
+        } else if (OUT && a.state) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            S[kt][t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (OUT && sg.n_seg > 1) {
-                S[kt][t] = mine[(kt * NT + t) * 256];
-            } else if (OUT && a.state) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) S[kt][t][j] = a.state[sbase + (size_t)(16 * kt + 4 * g + j) * DV + state_col<NT>(wave, n, t)];
-            }
+            for (int j = 0; j < 4; j++) S[kt][j] = a.state[sbase + (size_t)(16 * kt + 4 * g + j) * DV];
         }
+    }
     const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * DV;
     mk_v4u kr[KP], vr[VP], qr[OUT ? KP : 1];
     float gr;
     // A block's rows into registers: a scalar base, a lane offset that never changes, and a scalar step from piece to piece.  Rows behind the
     // sequence are read as its last one (and dropped at the store).
-    const int rk = threadIdx.x / (DK / E), rv = threadIdx.x / (DV / E), dk0 = threadIdx.x % (DK / E) * E, dv0 = threadIdx.x % (DV / E) * E;
     auto rows = [&](mk_v4u *dst, const T *base, size_t stride, int first, int r0, int d0, auto pieces, auto step) {
         const T *p = base + (size_t)(t0 + first) * stride;
         if (first + CH <= len) {
@@ -272,7 +264,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
             for (int i = 0; i < decltype(pieces)::value; i++) dst[i] = *(const mk_v4u *)(p + (size_t)min(r0 + i * decltype(step)::value, len - 1 - first) * stride + d0);
         }
     };
-    auto fetch = [&](int c) {
+    auto fetch = [&](int c, int tid) {
+        const int rk = tid / (DK / E), rv = tid / (DV / E), dk0 = tid % (DK / E) * E, dv0 = tid % (DV / E) * E;
         rows(kr, kp, a.ks, c * CH, rk, dk0, Int<KP>(), Int<CH / KP>());
         if constexpr (OUT) rows(qr, qp, a.qs, c * CH, rk, dk0, Int<KP>(), Int<CH / KP>());
         rows(vr, vp, a.vs, c * CH, rv, dv0, Int<VP>(), Int<CH / VP>());
@@ -289,8 +282,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
         total += end;
     };
     if (c0 < c1) {
-        fetch(c0);
-        if (wave == 0) {
+        fetch(c0, threadIdx.x);
+        if (wave == NW - 1) {
             scan(c0, decays(c0));
             gr = decays(c0 + 1);
         }
@@ -298,115 +291,112 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
     if (threadIdx.x == 0) bad_l = 0;
     for (int c = c0; c < c1; c++) {
         mk_wg_barrier();
+        // (addresses are formed anew in every block: held across it they would not fit the registers)
+        int n = lane & 15, g = lane >> 4, tid = threadIdx.x;
+        asm volatile("" : "+v"(n), "+v"(g), "+v"(tid));
+        const int rk = tid / (DK / E), rv = tid / (DV / E), dk0 = tid % (DK / E) * E, dv0 = tid % (DV / E) * E;
         bool ok = true;
         const int left = len - c * CH;  // tokens from this block on: behind them zeros, and no decay
         const mk_v4u zero = mk_v4u{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < KP; i++) {
-            const int at = i * 256 + threadIdx.x, r = at / (DK / E), d = at % (DK / E) * E;
-            *(mk_v4u *)&k_l[r * LK + d] = r < left ? kr[i] : zero;
-            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + d] = r < left ? qr[i] : zero;
+            const int r = rk + i * (CH / KP);
+            *(mk_v4u *)&k_l[r * LK + dk0] = r < left ? kr[i] : zero;
+            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + dk0] = r < left ? qr[i] : zero;
         }
 #pragma unroll
         for (int i = 0; i < VP; i++) {
-            const int at = i * 256 + threadIdx.x, r = at / (DV / E), d = at % (DV / E) * E;
+            const int r = rv + i * (CH / VP);
             const mk_v4u x = r < left ? vr[i] : zero;
-            *(mk_v4u *)&v_l[r * LV + d] = x;
+            *(mk_v4u *)&v_l[r * LV + dv0] = x;
             ok &= Op<T>::finite(x);
         }
         if (OUT && !ok) bad_l = c + 1;
         mk_wg_barrier();
-        if (c + 1 < c1) fetch(c + 1);
         const int u = c & 1;
         if constexpr (OUT) {
-            // scores of the wave's 16 query tokens
-            F qf[DK / 32];
+            // scores: operand f = (query tile j, 32 keys from 32 s2 on); the masked half of a diagonal one is not computed
+            for (int f = wave; f < 6; f += NW) {
+                const int j = f < 4 ? f : f - 2, s2 = f < 4 ? 0 : 1;
+                const double bq = b_l[u][16 * j + n];
+                F qf[KS];
 #pragma unroll
-            for (int s = 0; s < DK / 32; s++) qf[s] = row8(&q_l[(16 * wave + n) * LK + 32 * s + 8 * g]);
-            const double bq = b_l[u][16 * wave + n];
-            for (int s2 = 0; s2 <= wave / 2; s2++) {
+                for (int s = 0; s < KS; s++) qf[s] = row8(&q_l[(16 * j + n) * LK + 32 * s + 8 * g]);
                 mk_f4 pt[2];
 #pragma unroll
                 for (int v = 0; v < 2; v++) {
                     const int i = 2 * s2 + v;
                     pt[v] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (i <= wave) {
+                    if (i <= j) {
 #pragma unroll
-                        for (int s = 0; s < DK / 32; s++) pt[v] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[v]);
+                        for (int s = 0; s < KS; s++) pt[v] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[v]);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) pt[v][j] *= pow2(bq - b_l[u][16 * i + 4 * g + j]) * a.scale;
-                        if (i == wave) {
+                        for (int e = 0; e < 4; e++) pt[v][e] *= pow2(bq - b_l[u][16 * i + 4 * g + e]) * a.scale;
+                        if (i == j) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                if (4 * g + j > n) pt[v][j] = 0.0f;
+                            for (int e = 0; e < 4; e++)
+                                if (4 * g + e > n) pt[v][e] = 0.0f;
                         }
                     }
                 }
-                p_l[s2 == 0 ? wave : 2 + wave][lane] = operand<T>(pt[0], pt[1]);  // (second half: queries 32 .. 63 only)
+                p_l[f][lane] = operand<T>(pt[0], pt[1]);
             }
-            // (the wave with the fewest scores forms the next block's sums)
-            if (wave == 0 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
-            mk_wg_barrier();
-        } else {
-            if (wave == 0 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
         }
-        F vt[NT][2];
+        // (a wave with few or no scores forms the next block's sums)
+        if (wave == NW - 1 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
+        if constexpr (OUT) mk_wg_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        F vt[2];
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) vt[t][ks] = column8<LV, RUN>(v_l, ks, DV / 4 * wave + 4 * t * (NT - 1), g, n);
+        for (int ks = 0; ks < 2; ks++) vt[ks] = column8<LV>(v_l, ks, 16 * wave, g, n);
         if constexpr (OUT) {
             const bool plain = bad_l == c + 1;  // a value that is not finite: 0 times it must not reach earlier tokens
-            F sf[NT][DK / 32];
+            F sf[KS];
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int s = 0; s < KS; s++) sf[s] = operand<T>(S[2 * s], S[2 * s + 1]);
+            mk_f4 o[4];
 #pragma unroll
-                for (int s = 0; s < DK / 32; s++) sf[t][s] = operand<T>(S[2 * s][t], S[2 * s + 1][t]);
+            for (int j = 0; j < 4; j++) o[j] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row44(&q_l[(16 * j + n) * LK + 32 * s + 4 * g]), o[j]);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                F qb[DK / 32];
-#pragma unroll
-                for (int s = 0; s < DK / 32; s++) qb[s] = row44(&q_l[(16 * j + n) * LK + 32 * s + 4 * g]);
-                mk_f4 o[NT];
                 const float e = e_l[u][16 * j + n];
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    o[t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < 4; i++) o[j][i] *= e;
+            }
+            if (!plain) {
 #pragma unroll
-                    for (int s = 0; s < DK / 32; s++) o[t] = Op<T>::mma(sf[t][s], qb[s], o[t]);
+                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(vt[0], p_l[j][lane], o[j]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) o[t][i] *= e;
-                }
-                if (!plain) {
+                for (int j = 2; j < 4; j++) o[j] = Op<T>::mma(vt[1], p_l[2 + j][lane], o[j]);
+            } else {
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        o[t] = Op<T>::mma(vt[t][0], p_l[j][lane], o[t]);
-                        if (j >= 2) o[t] = Op<T>::mma(vt[t][1], p_l[2 + j][lane], o[t]);
-                    }
-                } else {
-                    const int tok = 16 * j + n;
-                    for (int key = 0; key <= tok; key++) {
+                for (int j = 0; j < 4; j++)
+                    for (int key = 0; key <= 16 * j + n; key++) {
                         const int r = key & 31;
                         const float p = (float)p_l[key < 32 ? j : 2 + j][16 * ((r & 15) >> 2) + n][4 * (r >> 4) + (r & 3)];
 #pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[t][i] = fmaf(p, (float)v_l[key * LV + state_col<NT>(wave, 4 * g + i, t)], o[t][i]);
+                        for (int i = 0; i < 4; i++) o[j][i] = fmaf(p, (float)v_l[key * LV + 16 * wave + 4 * g + i], o[j][i]);
                     }
-                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
                 const int tok = c * CH + 16 * j + n;
                 if (tok < len) {
-                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + state_col<NT>(wave, 4 * g, 0);
-                    if constexpr (NT == 2) {
-                        const mk_f4 lo = o[0], hi = o[1];
-                        if constexpr (sizeof(T) == 4) *(mk_f4 *)dst = lo, *(mk_f4 *)(dst + 4) = hi;
-                        else *(mk_b8 *)dst = operand<T>(lo, hi);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) dst[i] = (T)o[0][i];
-                    }
+                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + 16 * wave + 4 * g;
+                    if constexpr (sizeof(T) == 4) *(mk_f4 *)dst = o[j];
+                    else *(mk_b4 *)dst = mk_b4{(__bf16)o[j][0], (__bf16)o[j][1], (__bf16)o[j][2], (__bf16)o[j][3]};
                 }
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (the phases' registers do not add up)
+        if (c + 1 < c1) {
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));
+            fetch(c + 1, tid);
         }
         // the state behind the block
         if (!OUT || sg.n_seg == 1 || c + 1 < c1) {
@@ -414,85 +404,73 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void linear_block_kern
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) S[kt][t][j] *= end;
+                for (int j = 0; j < 4; j++) S[kt][j] *= end;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
-                F wv[NT][Op<T>::TERMS];
-                float w[8];
+                F wv[Op<T>::TERMS];
+                float w[8], r[8];
                 *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[u][32 * ks + 4 * g];
                 *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[u][32 * ks + 16 + 4 * g];
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    float r[8];
+                for (int i = 0; i < 8; i++) r[i] = (float)vt[ks][i] * w[i];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) r[i] = (float)vt[t][ks][i] * w[i];
+                for (int k = 0; k < Op<T>::TERMS; k++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        wv[k][i] = (T)r[i];
+                        r[i] -= (float)wv[k][i];
+                    }
+#pragma unroll
+                for (int kt = 0; kt < KT; kt += 2) {  // two sums in turn
+                    F kf[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) kf[i] = column8<LK>(k_l, ks, 16 * (kt + i), g, n);
 #pragma unroll
                     for (int k = 0; k < Op<T>::TERMS; k++)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            wv[t][k][i] = (T)r[i];
-                            r[i] -= (float)wv[t][k][i];
-                        }
-                }
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++) {
-                    const F kf = column8<LK, 4>(k_l, ks, 16 * kt, g, n);
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int k = 0; k < Op<T>::TERMS; k++) S[kt][t] = Op<T>::mma(kf, wv[t][k], S[kt][t]);
+                        for (int i = 0; i < 2; i++) S[kt + i] = Op<T>::mma(kf[i], wv[k], S[kt + i]);
                 }
             }
         }
     }
     if (OUT && sg.n_seg > 1) return;
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++)
+    for (int kt = 0; kt < KT; kt++) {
+        if constexpr (OUT) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            if constexpr (OUT) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) a.state_out[sbase + (size_t)(16 * kt + 4 * g + j) * DV + state_col<NT>(wave, n, t)] = S[kt][t][j];
-            } else {
-                mine[(kt * NT + t) * 256] = S[kt][t];
-            }
+            for (int j = 0; j < 4; j++) a.state_out[sbase + (size_t)(16 * kt + 4 * g + j) * DV] = S[kt][j];
+        } else {
+            mine[kt * TH] = S[kt];
         }
-    if (!OUT && threadIdx.x == 0) sg.decay[bh * sg.n_seg + seg] = pow2(total);
+    }
+    if (!OUT && threadIdx.x == TH - 1) sg.decay[bh * sg.n_seg + seg] = pow2(total);
 }
 
 // Between the two passes over the segments: local states -> the states before each segment, and the state behind the last.  One
-// workgroup: a quarter of the register tiles of (head, sequence).
+// workgroup: a tile of 16 rows of the state of (head, sequence).
 template <int DK, int DV>
-__global__ __launch_bounds__(256) void linear_carry_kernel(LinArgs a, LinSeg sg) {
-    constexpr int NT = DV / 64, TILES = DK / 16 * NT;
-    const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV;
+__global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg sg) {
+    constexpr int KT = DK / 16, TH = DV * 4;
+    const int kt = blockIdx.x, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const size_t bh = (size_t)b * a.nh + h, at = bh * DK * DV + (size_t)(16 * kt + 4 * g) * DV + 16 * wave + n;
     const int len = max(a.at(b + 1) - a.at(b), 0);
-    const int tile = blockIdx.x, kt = tile / NT, t = tile % NT;
     mk_f4 S = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    const size_t at = sbase + (size_t)(16 * kt + 4 * g) * DV + state_col<NT>(wave, n, t);
     if (a.state) {
 #pragma unroll
         for (int j = 0; j < 4; j++) S[j] = a.state[at + (size_t)j * DV];
     }
-    mk_f4 *p = sg.local + (bh * sg.n_seg * TILES + tile) * 256 + threadIdx.x;
-    for (int s0 = 0; s0 < sg.n_seg; s0 += 4) {
-        mk_f4 L[4];
-        float E[4];
-        bool has[4];
+    mk_f4 *p = sg.local + (bh * sg.n_seg * KT + kt) * TH + threadIdx.x;
+    const int nch = (len + CH - 1) / CH, per = (nch + sg.n_seg - 1) / sg.n_seg, used = per ? (nch + per - 1) / per : 0;  // (segment())
+    for (int s0 = 0; s0 < used; s0 += 8) {
+        mk_f4 L[8];
+        float E[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            int c0 = 0, c1 = 0;
-            if (s0 + i < sg.n_seg) segment(len, sg.n_seg, s0 + i, c0, c1);
-            has[i] = c0 < c1;
-            if (has[i]) L[i] = p[(size_t)(s0 + i) * TILES * 256], E[i] = sg.decay[bh * sg.n_seg + s0 + i];
-        }
+        for (int i = 0; i < 8; i++)
+            if (s0 + i < used) L[i] = p[(size_t)(s0 + i) * KT * TH], E[i] = sg.decay[bh * sg.n_seg + s0 + i];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (has[i]) {
-                p[(size_t)(s0 + i) * TILES * 256] = S;
+        for (int i = 0; i < 8; i++)
+            if (s0 + i < used) {
+                p[(size_t)(s0 + i) * KT * TH] = S;
 #pragma unroll
                 for (int j = 0; j < 4; j++) S[j] = fmaf(E[i], S[j], L[i][j]);
             }
@@ -515,15 +493,15 @@ bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv 
 
 template <typename T, int DK, int DV>
 int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
-    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B));
+    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B)), block(DV * 4);
     int e;
     if (sg.n_seg > 1) {
-        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, false>), grid, dim3(256), 0, st, a, sg);
+        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, false>), grid, block, 0, st, a, sg);
         if ((e = mk_launch_status("linear_block")) != MK_OK) return e;
-        hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16 * (DV / 64), (unsigned)a.nh, (unsigned)a.B), dim3(256), 0, st, a, sg);
+        hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16, (unsigned)a.nh, (unsigned)a.B), block, 0, st, a, sg);
         if ((e = mk_launch_status("linear_carry")) != MK_OK) return e;
     }
-    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, true>), grid, dim3(256), 0, st, a, sg);
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, true>), grid, block, 0, st, a, sg);
     return mk_launch_status("linear_block");
 }
 template <typename T>
