@@ -129,7 +129,8 @@ typedef float mk_f8v __attribute__((ext_vector_type(8)));
 template <typename T> struct Op;
 template <> struct Op<__bf16> {
     typedef mk_b8 F;
-    static constexpr int PAD = 8, TERMS = 3;
+    // values a row of K and V (read down the columns: eight rows of 4 + 4 words side by side) and of Q (read along the rows) is padded by
+    static constexpr int PAD = 16, QPAD = 8, TERMS = 3;
     static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ bool finite(const mk_v4u &r) {  // of a 16-byte piece of a row
         bool ok = true;
@@ -140,7 +141,7 @@ template <> struct Op<__bf16> {
 };
 template <> struct Op<float> {
     typedef mk_f8v F;
-    static constexpr int PAD = 4, TERMS = 1;
+    static constexpr int PAD = 4, QPAD = 4, TERMS = 1;
     static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) {
 #pragma unroll
         for (int i = 0; i < 8; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -209,22 +210,33 @@ __device__ __forceinline__ void segment(int n, int n_seg, int seg, int &c0, int 
 // 2^x for the decays: x is a difference of 64-bit sums of log2 decays, rounded once
 __device__ __forceinline__ float pow2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// inclusive sum over the wave in 64 bits
-__device__ __forceinline__ double wave_scan(double v, int lane) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(v, off, MK_WAVE);
-        if (lane >= off) v += o;
-    }
+// inclusive sum over the wave in 64 bits: within rows of 16 lanes by shifts, then the row before and the half before (all lanes active)
+template <int CTRL, int ROWS> __device__ __forceinline__ double shifted(double v) {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+    v += shifted<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);  // lane 15 of the row before, into rows 1 and 3
+    v += shifted<0x143, 0xC>(v);  // lane 31, into rows 2 and 3
     return v;
+}
+__device__ __forceinline__ double last_lane(double v) {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
 template <typename T, int DK, int DV, bool OUT>
 __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) : (OUT && DK > DV ? 1 : 2)) void linear_block_kernel(LinArgs a, LinSeg sg) {
     typedef typename Op<T>::F F;
-    constexpr int NW = DV / 16, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD;
+    constexpr int NW = DV / 16, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
-    __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LK : 8];
+    __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LQ : 8];
     __shared__ F p_l[OUT ? 6 : 1][64];                  // scores: query tiles 0 .. 3 with keys 0 .. 31, query tiles 2, 3 with keys 32 .. 63
     __shared__ double b_l[2][CH];                       // sums of the log2 decays of a block and of the next
     __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
@@ -274,7 +286,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
     double total = 0.0;
     auto scan = [&](int c, float gr) {  // one wave: the sums of block c
         const int u = c & 1;
-        const double s = wave_scan(c * CH + lane < len ? (double)(gr < -200.0f ? -200.0f : gr) * 1.4426950408889634 : 0.0, lane), end = __shfl(s, 63, MK_WAVE);
+        const double s = wave_scan(c * CH + lane < len ? (double)(gr < -200.0f ? -200.0f : gr) * 1.4426950408889634 : 0.0), end = last_lane(s);
         b_l[u][lane] = s;
         w_l[u][lane] = pow2(end - s);
         e_l[u][lane] = pow2(s) * a.scale;
@@ -302,7 +314,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
         for (int i = 0; i < KP; i++) {
             const int r = rk + i * (CH / KP);
             *(mk_v4u *)&k_l[r * LK + dk0] = r < left ? kr[i] : zero;
-            if constexpr (OUT) *(mk_v4u *)&q_l[r * LK + dk0] = r < left ? qr[i] : zero;
+            if constexpr (OUT) *(mk_v4u *)&q_l[r * LQ + dk0] = r < left ? qr[i] : zero;
         }
 #pragma unroll
         for (int i = 0; i < VP; i++) {
@@ -321,7 +333,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
                 const double bq = b_l[u][16 * j + n];
                 F qf[KS];
 #pragma unroll
-                for (int s = 0; s < KS; s++) qf[s] = row8(&q_l[(16 * j + n) * LK + 32 * s + 8 * g]);
+                for (int s = 0; s < KS; s++) qf[s] = row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]);
                 mk_f4 pt[2];
 #pragma unroll
                 for (int v = 0; v < 2; v++) {
@@ -360,7 +372,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row44(&q_l[(16 * j + n) * LK + 32 * s + 4 * g]), o[j]);
+                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row44(&q_l[(16 * j + n) * LQ + 32 * s + 4 * g]), o[j]);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float e = e_l[u][16 * j + n];
