@@ -177,6 +177,14 @@ __device__ __forceinline__ mk_f8v row44(const float *p) {
     const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 16);
     return mk_f8v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
+// A 16-byte piece of a query row (values d ..) into its LDS row, whose 32-value groups hold the values in operand order: lane group g's {4 g .. ,
+// 16 + 4 g ..} side by side, so that the operand is one read.
+__device__ __forceinline__ void store_q(__bf16 *row, int d, const mk_v4u &x) {
+    __bf16 *p = row + (d & ~31) + 8 * ((d & 15) >> 2) + 4 * ((d & 31) >> 4);
+    *(mk_u2 *)p = mk_u2{x[0], x[1]};
+    *(mk_u2 *)(p + 8) = mk_u2{x[2], x[3]};
+}
+__device__ __forceinline__ void store_q(float *row, int d, const mk_v4u &x) { *(mk_v4u *)(row + (d & ~31) + 8 * ((d & 15) >> 2) + 4 * ((d & 31) >> 4)) = x; }
 // a transposed operand of a tile in LDS [token][LD]: lane (g, n) gets column cols + n of the tokens 32 ks + 4 g .. + 3 and 16 further
 template <int LD> __device__ __forceinline__ mk_b8 column8(const __bf16 *tile, int ks, int cols, int g, int n) {
     typedef short s4 __attribute__((ext_vector_type(4)));
@@ -231,9 +239,13 @@ __device__ __forceinline__ double last_lane(double v) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-template <typename T, int DK, int DV, bool OUT>
-__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) : (OUT && DK > DV ? 1 : 2)) void linear_block_kernel(LinArgs a, LinSeg sg) {
+enum Mode { LOCAL, OUTPUT, BOTH };  // local states of the segments; outputs from the states before them; one segment: outputs and state
+template <typename T, int DK, int DV, Mode MODE>
+__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV ? 2 : 4) : (MODE != LOCAL && DK > DV ? 1 : 2)) void linear_block_kernel(LinArgs a, LinSeg sg) {
     typedef typename Op<T>::F F;
+    constexpr bool OUT = MODE != LOCAL;
+    // the state that only leads to the next outputs takes two terms (2^-17 beside its own rounding to bfloat16)
+    constexpr int TERMS = MODE == OUTPUT && Op<T>::TERMS > 2 ? 2 : Op<T>::TERMS;
     constexpr int NW = DV / 16, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
     __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LQ : 8];
@@ -253,9 +265,9 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
         S[kt] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (OUT && sg.n_seg > 1) {
+        if (MODE == OUTPUT) {
             S[kt] = mine[kt * TH];
-        } else if (OUT && a.state) {
+        } else if (MODE == BOTH && a.state) {
 #pragma unroll
             for (int j = 0; j < 4; j++) S[kt][j] = a.state[sbase + (size_t)(16 * kt + 4 * g + j) * DV];
         }
@@ -314,7 +326,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
         for (int i = 0; i < KP; i++) {
             const int r = rk + i * (CH / KP);
             *(mk_v4u *)&k_l[r * LK + dk0] = r < left ? kr[i] : zero;
-            if constexpr (OUT) *(mk_v4u *)&q_l[r * LQ + dk0] = r < left ? qr[i] : zero;
+            if constexpr (OUT) store_q(&q_l[r * LQ], dk0, r < left ? qr[i] : zero);
         }
 #pragma unroll
         for (int i = 0; i < VP; i++) {
@@ -341,7 +353,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
                     pt[v] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
                     if (i <= j) {
 #pragma unroll
-                        for (int s = 0; s < KS; s++) pt[v] = Op<T>::mma(row8(&k_l[(16 * i + n) * LK + 32 * s + 8 * g]), qf[s], pt[v]);
+                        for (int s = 0; s < KS; s++) pt[v] = Op<T>::mma(row44(&k_l[(16 * i + n) * LK + 32 * s + 4 * g]), qf[s], pt[v]);
 #pragma unroll
                         for (int e = 0; e < 4; e++) pt[v][e] *= pow2(bq - b_l[u][16 * i + 4 * g + e]) * a.scale;
                         if (i == j) {
@@ -372,7 +384,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row44(&q_l[(16 * j + n) * LQ + 32 * s + 4 * g]), o[j]);
+                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]), o[j]);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float e = e_l[u][16 * j + n];
@@ -411,7 +423,7 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
             fetch(c + 1, tid);
         }
         // the state behind the block
-        if (!OUT || sg.n_seg == 1 || c + 1 < c1) {
+        if (MODE != OUTPUT || c + 1 < c1) {
             const float end = last_l[u];
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
@@ -419,14 +431,14 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
                 for (int j = 0; j < 4; j++) S[kt][j] *= end;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
-                F wv[Op<T>::TERMS];
+                F wv[TERMS];
                 float w[8], r[8];
                 *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[u][32 * ks + 4 * g];
                 *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[u][32 * ks + 16 + 4 * g];
 #pragma unroll
                 for (int i = 0; i < 8; i++) r[i] = (float)vt[ks][i] * w[i];
 #pragma unroll
-                for (int k = 0; k < Op<T>::TERMS; k++)
+                for (int k = 0; k < TERMS; k++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         wv[k][i] = (T)r[i];
@@ -438,24 +450,24 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (OUT && DK > DV ? 2 : 4) :
 #pragma unroll
                     for (int i = 0; i < 2; i++) kf[i] = column8<LK>(k_l, ks, 16 * (kt + i), g, n);
 #pragma unroll
-                    for (int k = 0; k < Op<T>::TERMS; k++)
+                    for (int k = 0; k < TERMS; k++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) S[kt + i] = Op<T>::mma(kf[i], wv[k], S[kt + i]);
                 }
             }
         }
     }
-    if (OUT && sg.n_seg > 1) return;
+    if (MODE == OUTPUT) return;
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
-        if constexpr (OUT) {
+        if constexpr (MODE == BOTH) {
 #pragma unroll
             for (int j = 0; j < 4; j++) a.state_out[sbase + (size_t)(16 * kt + 4 * g + j) * DV] = S[kt][j];
         } else {
             mine[kt * TH] = S[kt];
         }
     }
-    if (!OUT && threadIdx.x == TH - 1) sg.decay[bh * sg.n_seg + seg] = pow2(total);
+    if (MODE == LOCAL && threadIdx.x == TH - 1) sg.decay[bh * sg.n_seg + seg] = pow2(total);
 }
 
 // Between the two passes over the segments: local states -> the states before each segment, and the state behind the last.  One
@@ -507,13 +519,15 @@ template <typename T, int DK, int DV>
 int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
     const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B)), block(DV * 4);
     int e;
-    if (sg.n_seg > 1) {
-        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, false>), grid, block, 0, st, a, sg);
-        if ((e = mk_launch_status("linear_block")) != MK_OK) return e;
-        hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16, (unsigned)a.nh, (unsigned)a.B), block, 0, st, a, sg);
-        if ((e = mk_launch_status("linear_carry")) != MK_OK) return e;
+    if (sg.n_seg == 1) {
+        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, BOTH>), grid, block, 0, st, a, sg);
+        return mk_launch_status("linear_block");
     }
-    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, true>), grid, block, 0, st, a, sg);
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, LOCAL>), grid, block, 0, st, a, sg);
+    if ((e = mk_launch_status("linear_block")) != MK_OK) return e;
+    hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16, (unsigned)a.nh, (unsigned)a.B), block, 0, st, a, sg);
+    if ((e = mk_launch_status("linear_carry")) != MK_OK) return e;
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, OUTPUT>), grid, block, 0, st, a, sg);
     return mk_launch_status("linear_block");
 }
 template <typename T>
