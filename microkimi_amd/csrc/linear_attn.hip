@@ -113,8 +113,8 @@ int launch_token(const LinArgs &a, hipStream_t st) {
 // which is all matrix products, and every exponent of the decays is a difference of sums of the same block: formed in 64 bits, so that
 // no large sum cancels, it is never positive for log decays that are not (a log decay below -200 counts as -200: e^-200 is 0).
 //
-// One workgroup: a run of blocks of (value head, sequence), one wave for every 16 columns of dv.  The state stays in registers across the
-// blocks, as the matrix instruction returns it: tile kt of S = rows 16 kt + 4 g + j, the wave's column n (lane = 16 g + n).  Two such
+// One workgroup: a run of blocks of (value head, sequence), one wave for every 16 or 32 columns of dv.  The state stays in registers across the
+// blocks, as the matrix instruction returns it: tile kt of S = rows 16 kt + 4 g + j, column n of 16 (lane = 16 g + n).  Two such
 // tiles ARE an operand of the next product once the sum over dk takes its terms in the order {4 g .. , 16 + 4 g ..}; the same
 // holds for the block's scores and the sum over its tokens.  So the waves exchange only the scores, through LDS in operand order:
 //   scores   A = K rows, B = Q rows               -> (key, query), weighted by the decay, masked, to LDS (six operands, shared out)
@@ -240,13 +240,16 @@ __device__ __forceinline__ double last_lane(double v) {
 }
 
 enum Mode { LOCAL, OUTPUT, BOTH };  // local states of the segments; outputs from the states before them; one segment: outputs and state
+// NT: tiles of 16 columns a wave.  Two (a wave's operands of Q, K and the scores, read from LDS, serve both) where the reads bound it: with one, 16
+// waves a compute unit read 16 KB of queries each block.  One for the local states, whose four waves a SIMD hide more.
+template <typename T, int DK, int DV, Mode MODE> constexpr int tiles() { return MODE != LOCAL && sizeof(T) == 2 && DV == 128 ? 2 : 1; }
 template <typename T, int DK, int DV, Mode MODE>
-__global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV ? 2 : 4) : (MODE != LOCAL && DK > DV ? 1 : 2)) void linear_block_kernel(LinArgs a, LinSeg sg) {
+__global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 4 && DK > DV ? 1 : 2) void linear_block_kernel(LinArgs a, LinSeg sg) {
     typedef typename Op<T>::F F;
     constexpr bool OUT = MODE != LOCAL;
     // the state that only leads to the next outputs takes two terms (2^-17 beside its own rounding to bfloat16)
     constexpr int TERMS = MODE == OUTPUT && Op<T>::TERMS > 2 ? 2 : Op<T>::TERMS;
-    constexpr int NW = DV / 16, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
+    constexpr int NT = tiles<T, DK, DV, MODE>(), NW = DV / 16 / NT, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
     __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LQ : 8];
     __shared__ F p_l[OUT ? 6 : 1][64];                  // scores: query tiles 0 .. 3 with keys 0 .. 31, query tiles 2, 3 with keys 32 .. 63
@@ -258,20 +261,22 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV 
     const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0);
     int c0, c1;
     segment(len, sg.n_seg, seg, c0, c1);
-    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV + 16 * wave + n;
+    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV + 16 * NT * wave + n;
     if (c0 >= c1 && sg.n_seg > 1) return;
-    mk_f4 S[KT];
-    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT) * TH + threadIdx.x;
+    mk_f4 S[KT][NT];
+    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT) * (DV * 4) + 64 * NT * wave + lane;
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-        S[kt] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (MODE == OUTPUT) {
-            S[kt] = mine[kt * TH];
-        } else if (MODE == BOTH && a.state) {
+    for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) S[kt][j] = a.state[sbase + (size_t)(16 * kt + 4 * g + j) * DV];
+        for (int t = 0; t < NT; t++) {
+            S[kt][t] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (MODE == OUTPUT) {
+                S[kt][t] = mine[kt * (DV * 4) + 64 * t];
+            } else if (MODE == BOTH && a.state) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) S[kt][t][j] = a.state[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * DV];
+            }
         }
-    }
     const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * DV;
     mk_v4u kr[KP], vr[VP], qr[OUT ? KP : 1];
     float gr;
@@ -340,7 +345,8 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV 
         const int u = c & 1;
         if constexpr (OUT) {
             // scores: operand f = (query tile j, 32 keys from 32 s2 on); the masked half of a diagonal one is not computed
-            for (int f = wave; f < 6; f += NW) {
+            for (int i = wave; i < 6; i += NW) {
+                const int f = NW == 4 ? (0x405321 >> (4 * i)) & 15 : i;  // (of four waves: 1 + 0, 2 + 4, 3, 5)
                 const int j = f < 4 ? f : f - 2, s2 = f < 4 ? 0 : 1;
                 const double bq = b_l[u][16 * j + n];
                 F qf[KS];
@@ -370,32 +376,42 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV 
         if (wave == NW - 1 && c + 1 < c1) scan(c + 1, gr), gr = decays(c + 2);
         if constexpr (OUT) mk_wg_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        F vt[2];
+        F vt[NT][2];
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) vt[ks] = column8<LV>(v_l, ks, 16 * wave, g, n);
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) vt[t][ks] = column8<LV>(v_l, ks, 16 * (NT * wave + t), g, n);
         if constexpr (OUT) {
             const bool plain = bad_l == c + 1;  // a value that is not finite: 0 times it must not reach earlier tokens
-            F sf[KS];
+            F sf[NT][KS];
 #pragma unroll
-            for (int s = 0; s < KS; s++) sf[s] = operand<T>(S[2 * s], S[2 * s + 1]);
-            mk_f4 o[4];
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int s = 0; s < KS; s++) sf[t][s] = operand<T>(S[2 * s][t], S[2 * s + 1][t]);
+            mk_f4 o[NT][4];
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(sf[s], row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]), o[j]);
+                for (int j = 0; j < 4; j++) {
+                    const F qb = row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) o[t][j] = Op<T>::mma(sf[t][s], qb, s ? o[t][j] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
+                }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float e = e_l[u][16 * j + n];
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[j][i] *= e;
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t][j][i] *= e;
             }
             if (!plain) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = Op<T>::mma(vt[0], p_l[j][lane], o[j]);
+                for (int f = 0; f < 6; f++) {
+                    const F pb = p_l[f][lane];
 #pragma unroll
-                for (int j = 2; j < 4; j++) o[j] = Op<T>::mma(vt[1], p_l[2 + j][lane], o[j]);
+                    for (int t = 0; t < NT; t++) o[t][f < 4 ? f : f - 2] = Op<T>::mma(vt[t][f < 4 ? 0 : 1], pb, o[t][f < 4 ? f : f - 2]);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
@@ -403,16 +419,22 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV 
                         const int r = key & 31;
                         const float p = (float)p_l[key < 32 ? j : 2 + j][16 * ((r & 15) >> 2) + n][4 * (r >> 4) + (r & 3)];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[j][i] = fmaf(p, (float)v_l[key * LV + 16 * wave + 4 * g + i], o[j][i]);
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[t][j][i] = fmaf(p, (float)v_l[key * LV + 16 * (NT * wave + t) + 4 * g + i], o[t][j][i]);
                     }
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int tok = c * CH + 16 * j + n;
                 if (tok < len) {
-                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + 16 * wave + 4 * g;
-                    if constexpr (sizeof(T) == 4) *(mk_f4 *)dst = o[j];
-                    else *(mk_b4 *)dst = mk_b4{(__bf16)o[j][0], (__bf16)o[j][1], (__bf16)o[j][2], (__bf16)o[j][3]};
+                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + 16 * NT * wave + 4 * g;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const mk_f4 x = o[t][j];
+                        if constexpr (sizeof(T) == 4) *(mk_f4 *)(dst + 16 * t) = x;
+                        else *(mk_b4 *)(dst + 16 * t) = mk_b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+                    }
                 }
             }
         }
@@ -428,45 +450,55 @@ __global__ __launch_bounds__(DV * 4, sizeof(T) == 2 ? (MODE != LOCAL && DK > DV 
 #pragma unroll
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) S[kt][j] *= end;
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) S[kt][t][j] *= end;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
-                F wv[TERMS];
-                float w[8], r[8];
+                F wv[NT][TERMS];
+                float w[8];
                 *(mk_f4 *)&w[0] = *(const mk_f4 *)&w_l[u][32 * ks + 4 * g];
                 *(mk_f4 *)&w[4] = *(const mk_f4 *)&w_l[u][32 * ks + 16 + 4 * g];
 #pragma unroll
-                for (int i = 0; i < 8; i++) r[i] = (float)vt[ks][i] * w[i];
+                for (int t = 0; t < NT; t++) {
+                    float r[8];
 #pragma unroll
-                for (int k = 0; k < TERMS; k++)
+                    for (int i = 0; i < 8; i++) r[i] = (float)vt[t][ks][i] * w[i];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        wv[k][i] = (T)r[i];
-                        r[i] -= (float)wv[k][i];
-                    }
+                    for (int k = 0; k < TERMS; k++)
 #pragma unroll
-                for (int kt = 0; kt < KT; kt += 2) {  // two sums in turn
+                        for (int i = 0; i < 8; i++) {
+                            wv[t][k][i] = (T)r[i];
+                            r[i] -= (float)wv[t][k][i];
+                        }
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; kt += 2) {  // several sums in turn
                     F kf[2];
 #pragma unroll
                     for (int i = 0; i < 2; i++) kf[i] = column8<LK>(k_l, ks, 16 * (kt + i), g, n);
 #pragma unroll
                     for (int k = 0; k < TERMS; k++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) S[kt + i] = Op<T>::mma(kf[i], wv[k], S[kt + i]);
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int t = 0; t < NT; t++) S[kt + i][t] = Op<T>::mma(kf[i], wv[t][k], S[kt + i][t]);
                 }
             }
         }
     }
     if (MODE == OUTPUT) return;
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-        if constexpr (MODE == BOTH) {
+    for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) a.state_out[sbase + (size_t)(16 * kt + 4 * g + j) * DV] = S[kt][j];
-        } else {
-            mine[kt * TH] = S[kt];
+        for (int t = 0; t < NT; t++) {
+            if constexpr (MODE == BOTH) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) a.state_out[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * DV] = S[kt][t][j];
+            } else {
+                mine[kt * (DV * 4) + 64 * t] = S[kt][t];
+            }
         }
-    }
     if (MODE == LOCAL && threadIdx.x == TH - 1) sg.decay[bh * sg.n_seg + seg] = pow2(total);
 }
 
@@ -517,17 +549,17 @@ bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv 
 
 template <typename T, int DK, int DV>
 int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
-    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B)), block(DV * 4);
+    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B));
     int e;
     if (sg.n_seg == 1) {
-        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, BOTH>), grid, block, 0, st, a, sg);
+        hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, BOTH>), grid, dim3(DV * 4 / tiles<T, DK, DV, BOTH>()), 0, st, a, sg);
         return mk_launch_status("linear_block");
     }
-    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, LOCAL>), grid, block, 0, st, a, sg);
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, LOCAL>), grid, dim3(DV * 4 / tiles<T, DK, DV, LOCAL>()), 0, st, a, sg);
     if ((e = mk_launch_status("linear_block")) != MK_OK) return e;
-    hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16, (unsigned)a.nh, (unsigned)a.B), block, 0, st, a, sg);
+    hipLaunchKernelGGL((linear_carry_kernel<DK, DV>), dim3(DK / 16, (unsigned)a.nh, (unsigned)a.B), dim3(DV * 4), 0, st, a, sg);
     if ((e = mk_launch_status("linear_carry")) != MK_OK) return e;
-    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, OUTPUT>), grid, block, 0, st, a, sg);
+    hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, OUTPUT>), grid, dim3(DV * 4 / tiles<T, DK, DV, OUTPUT>()), 0, st, a, sg);
     return mk_launch_status("linear_block");
 }
 template <typename T>
