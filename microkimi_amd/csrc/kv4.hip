@@ -14,97 +14,138 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------------------ append
 
-// One wave: 64 items of a row of the call.  An item is 8 values: nkv * dk / 8 of K, nkv * dv / 8 of V, rope / 8 of the K tail.
-// dk and dv are multiples of 32, so a block of 32 values is an aligned quad of lanes.
-template <typename T>
+// Positions held after the rows [first, last) of a call; far beyond every capacity the count stays where it is.
+__device__ __forceinline__ int advanced(int held, int n) { return (int)min((int64_t)held + max(n, 0), (int64_t)1 << 30); }
+
+// Two rows a wave: 6340 rows of 2048 values 12.3 us (four rows the same, one row 14.8), 16 rows of one token 5.0 us (four rows 6.8, one 3.8).
+constexpr int APPEND_ROWS = 2;
+
+// One wave: 64 items of ROWS rows of the call.  An item is 8 values: nkv * dk / 8 of K, nkv * dv / 8 of V, rope / 8 of the K tail.
+// dk and dv are multiples of 32, so a block of 32 values is an aligned quad of lanes.  Levels come from v_cvt_scalef32_pk_fp4_f32,
+// which rounds a midpoint to the even code: half of the midpoints go down.  With the lowest mantissa bit set first a midpoint is just
+// above itself, and no other value reaches or passes one (their lowest bit is clear), so every midpoint goes up.
+// When `fresh`, no row reads lens, and the last workgroup writes them; otherwise kv4_advance_kernel does behind this one.
+template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void kv4_append_kernel(MkKv4 c, MkSeqs s, const T *__restrict__ k_rows, size_t k_stride, const T *__restrict__ v_rows,
                                                          size_t v_stride, int fresh, int waves_per_row) {
-    const int w = (int)(blockIdx.x * 4 + (threadIdx.x >> 6));
-    const int t = w / waves_per_row;
-    if (t >= s.T) return;
-    const int b = s.of_row(t);
-    if (b < 0) return;
-    const int pos = (fresh ? 0 : c.lens[b]) + (t - s.at(b));
-    if (pos < 0 || pos >= c.cap) return;
-    const int item = (w - t * waves_per_row) * 64 + (threadIdx.x & 63);
+    if (fresh && blockIdx.x == gridDim.x - 1) {
+        for (int b = threadIdx.x; b < c.B; b += 256) c.lens[b] = advanced(0, s.at(b + 1) - s.at(b));
+        return;
+    }
+    const int w = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int t0 = w / waves_per_row * ROWS;
+    if (t0 >= s.T) return;
+    const int item = (w % waves_per_row) * 64 + (threadIdx.x & 63);
     const int nk = c.nkv * c.dk / 8, nv = c.nkv * c.dv / 8;
-    float v[8];
-    if (item < nk + nv) {
-        const bool is_v = item >= nk;
-        const int width = is_v ? c.dv : c.dk, e = (is_v ? item - nk : item) * 8;
-        const int h = e / width, d = e - h * width;
-        if (is_v) mk_load8(v_rows + (size_t)t * v_stride + (size_t)h * c.dv + d, v);
-        else mk_load8(k_rows + (size_t)t * k_stride + (size_t)h * (c.dk + c.rope) + d, v);
-        float m = 0.0f;
+    const bool coded = item < nk + nv, is_v = coded && item >= nk, tail = !coded && item < nk + nv + c.rope / 8;
+    const int width = is_v ? c.dv : c.dk, e = (is_v ? item - nk : item) * 8;
+    const int h = coded ? e / width : 0, d = coded ? e - h * width : (item - nk - nv) * 8;
+    const T *src = is_v ? v_rows + (size_t)h * c.dv + d : k_rows + (coded ? (size_t)h * (c.dk + c.rope) + d : (size_t)c.dk + d);
+    const size_t stride = is_v ? v_stride : k_stride;
+    float v[ROWS][8];  // every row is asked for before the first sequence is looked up
+    if (coded || tail) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-        m = fmaxf(m, mk_dpp<0xB1>(m));
-        m = fmaxf(m, mk_dpp<0x4E>(m));
-        const uint32_t bits = __float_as_uint(m);
-        int ex = (int)(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 2);
-        ex = max(-127, min(125, ex));
-        const float inv = mk_scale_from_byte((uint32_t)(127 - ex));
-        uint32_t code = 0;
+        for (int r = 0; r < ROWS; r++) mk_load8(src + (size_t)min(t0 + r, s.T - 1) * stride, v[r]);
+    }
+    int b = -1, first = 0, next = 0, held = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float a = fabsf(v[i]) * inv;
-            const uint32_t lev = (a >= 0.25f) + (a >= 0.75f) + (a >= 1.25f) + (a >= 1.75f) + (a >= 2.5f) + (a >= 3.5f) + (a >= 5.0f);
-            code |= (lev | (v[i] < 0.0f ? 8u : 0u)) << (4 * i);
+    for (int r = 0; r < ROWS; r++) {
+        const int t = t0 + r;
+        if (b < 0 || t >= next) {
+            b = t < s.T ? s.of_row(t) : -1;
+            if (b >= 0) first = s.at(b), next = s.at(b + 1), held = fresh ? 0 : min(c.lens[b], 1 << 30);
         }
-        const size_t row = ((size_t)b * c.nkv + h) * c.cap + pos;
-        uint8_t *q = is_v ? c.vq : c.kq, *sc = is_v ? c.vs : c.ks;
-        *(uint32_t *)(q + row * (width / 2) + d / 2) = code;
-        if ((item & 3) == 0) sc[row * (width / 32) + d / 32] = (uint8_t)(ex + 127);
-    } else if (item < nk + nv + c.rope / 8) {
-        const int d = (item - nk - nv) * 8;
-        mk_load8(k_rows + (size_t)t * k_stride + c.dk + d, v);
-        mk_b8 o;
+        const int pos = held + t - first;
+        if (b >= 0 && pos >= 0 && pos < c.cap) {
+            if (coded) {
+                float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = (__bf16)v[i];
-        *(mk_b8 *)(c.kr + ((size_t)b * c.cap + pos) * c.rope + d) = o;
+                for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[r][i]));
+                m = fmaxf(m, mk_dpp<0xB1>(m));
+                m = fmaxf(m, mk_dpp<0x4E>(m));
+                const uint32_t bits = __float_as_uint(m);
+                int ex = (int)(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 2);
+                ex = max(-127, min(125, ex));
+                const float inv = mk_scale_from_byte((uint32_t)(127 - ex));
+                float a[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = v[r][i] == v[r][i] ? (v[r][i] + 0.0f) * inv : 0.0f;  // (-0 becomes 0; a negative value that underflows keeps its sign)
+                    a[i] = __uint_as_float(__float_as_uint(x) | 1u);
+                }
+                uint32_t code = 0;
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, a[0], a[1], 1.0f, 0);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, a[2], a[3], 1.0f, 1);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, a[4], a[5], 1.0f, 2);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, a[6], a[7], 1.0f, 3);
+                const size_t row = ((size_t)b * c.nkv + h) * c.cap + pos;
+                uint8_t *q = is_v ? c.vq : c.kq, *sc = is_v ? c.vs : c.ks;
+                *(uint32_t *)(q + row * (width / 2) + d / 2) = code;
+                if ((item & 3) == 0) sc[row * (width / 32) + d / 32] = (uint8_t)(ex + 127);
+            } else if (tail) {
+                mk_b8 o;
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = (__bf16)v[r][i];
+                *(mk_b8 *)(c.kr + ((size_t)b * c.cap + pos) * c.rope + d) = o;
+            }
+        }
     }
 }
 
 __global__ __launch_bounds__(256) void kv4_advance_kernel(MkKv4 c, MkSeqs s, int fresh) {
     const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < c.B) c.lens[b] = (fresh ? 0 : c.lens[b]) + max(s.at(b + 1) - s.at(b), 0);
+    if (b < c.B) c.lens[b] = advanced(fresh ? 0 : c.lens[b], s.at(b + 1) - s.at(b));
 }
 
 // ------------------------------------------------------------------------------------------------------------ to_f32
 
-// One thread: 8 values of K or V of (sequence, position, head); positions a sequence does not hold are zero.
-__global__ __launch_bounds__(256) void kv4_to_f32_kernel(MkKv4 c, int n, float *__restrict__ k, float *__restrict__ v, int items, size_t total) {
-    const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= total) return;
-    const int item = (int)(idx % items);
-    const size_t row = idx / items;  // (b * n + pos) * nkv + h
-    const int h = (int)(row % c.nkv);
-    const size_t bp = row / c.nkv;
-    const int pos = (int)(bp % n), b = (int)(bp / n);
-    const bool held = pos < c.lens[b];
-    const int nk = c.dk / 8, nr = c.rope / 8;
-    float o[8];
+// HBM-bound: four sequences of 2048 positions of 8 heads of 128 + 128 (67 MB written) 13.7 us, the rate of a large copy.
+// One workgroup: SNAP positions of a sequence, a thread 4 values at a time (a wave stores 1 KiB in a row); positions a sequence does
+// not hold are zero.
+constexpr int SNAP = 4;
+
+__global__ __launch_bounds__(256) void kv4_to_f32_kernel(MkKv4 c, int n, float *__restrict__ k, float *__restrict__ v) {
+    const int b = blockIdx.y, p0 = blockIdx.x * SNAP;
+    const int len = c.lens[b], wk = c.dk + c.rope, nk = c.nkv * wk / 4, nv = c.nkv * c.dv / 4;
+    for (int item = threadIdx.x; item < nk + nv; item += 256) {
+        const bool is_v = item >= nk;
+        const int e = (is_v ? item - nk : item) * 4, across = is_v ? c.dv : wk, h = e / across, d = e - h * across;
+        const bool tail = !is_v && d >= c.dk;
+        const int width = is_v ? c.dv : c.dk;
+        const size_t at = ((size_t)b * c.nkv + h) * c.cap + p0;
+        const uint8_t *codes = (is_v ? c.vq : c.kq) + at * (width / 2) + d / 2, *scales = (is_v ? c.vs : c.ks) + at * (width / 32) + d / 32;
+        float *dst = (is_v ? v : k) + ((size_t)b * n + p0) * c.nkv * across + e;
+        mk_f4 o[SNAP];
+        if (tail) {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = 0.0f;
-    float *dst;
-    const size_t at = ((size_t)b * c.nkv + h) * c.cap + pos;
-    if (item >= nk && item < nk + nr) {
-        const int d = (item - nk) * 8;
-        dst = k + row * (c.dk + c.rope) + c.dk + d;
-        if (held) mk_load8((const __bf16 *)(c.kr + ((size_t)b * c.cap + pos) * c.rope + d), o);
-    } else {
-        const bool is_v = item >= nk + nr;
-        const int d = (is_v ? item - nk - nr : item) * 8, width = is_v ? c.dv : c.dk;
-        dst = is_v ? v + row * c.dv + d : k + row * (c.dk + c.rope) + d;
-        if (held) {
-            const uint32_t code = *(const uint32_t *)((is_v ? c.vq : c.kq) + at * (width / 2) + d / 2);
-            const float sc = mk_scale_from_byte((is_v ? c.vs : c.ks)[at * (width / 32) + d / 32]);
+            for (int p = 0; p < SNAP; p++) {
+                o[p] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (p0 + p < min(len, n)) {
+                    const b4 x = *(const b4 *)(c.kr + ((size_t)b * c.cap + p0 + p) * c.rope + d - c.dk);
+                    o[p] = mk_f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+                }
+            }
+        } else {
+            uint32_t code[SNAP], byte[SNAP];
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[i] = mk_e2m1((code >> (4 * i)) & 15u) * sc;
+            for (int p = 0; p < SNAP; p++) {
+                code[p] = byte[p] = 0;
+                if (p0 + p < min(len, n)) code[p] = *(const uint16_t *)(codes + (size_t)p * (width / 2)), byte[p] = scales[(size_t)p * (width / 32)];
+            }
+#pragma unroll
+            for (int p = 0; p < SNAP; p++) {
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                const float sc = mk_scale_from_byte(byte[p]);
+                const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 0), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 1);
+                o[p] = mk_f4{x[0] * sc, x[1] * sc, y[0] * sc, y[1] * sc};
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < SNAP; p++) {
+            if (p0 + p < n) __builtin_nontemporal_store(o[p], (mk_f4 *)(dst + (size_t)p * c.nkv * across));
         }
     }
-    *(mk_f4 *)dst = mk_f4{o[0], o[1], o[2], o[3]};
-    *(mk_f4 *)(dst + 4) = mk_f4{o[4], o[5], o[6], o[7]};
 }
 
 }  // namespace
@@ -121,14 +162,14 @@ extern "C" int mk_dev_kv4_append(const mk_kv4_cache *c, int dtype, const void *k
     const size_t items = c->nkv * (c->dk + c->dv) / 8 + c->rope / 8, wpr = (items + 63) / 64;
     MK_REQUIRE(T * wpr <= 0x7FFFFFFFull / 64, "too many rows in one call");
     if (T) {
-        const unsigned grid = (unsigned)((T * wpr + 3) / 4);
+        const size_t grid = ((T + APPEND_ROWS - 1) / APPEND_ROWS * wpr + 3) / 4 + (fresh ? 1 : 0);
         if (dtype == MK_F32)
-            hipLaunchKernelGGL(kv4_append_kernel<float>, dim3(grid), dim3(256), 0, (hipStream_t)stream, v, s, (const float *)k_rows, k_stride, (const float *)v_rows,
-                               v_stride, fresh, (int)wpr);
+            hipLaunchKernelGGL((kv4_append_kernel<float, APPEND_ROWS>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, v, s, (const float *)k_rows, k_stride,
+                               (const float *)v_rows, v_stride, fresh, (int)wpr);
         else
-            hipLaunchKernelGGL(kv4_append_kernel<__bf16>, dim3(grid), dim3(256), 0, (hipStream_t)stream, v, s, (const __bf16 *)k_rows, k_stride,
-                               (const __bf16 *)v_rows, v_stride, fresh, (int)wpr);
-        if ((st = mk_launch_status("kv4_append")) != MK_OK) return st;
+            hipLaunchKernelGGL((kv4_append_kernel<__bf16, APPEND_ROWS>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, v, s, (const __bf16 *)k_rows,
+                               k_stride, (const __bf16 *)v_rows, v_stride, fresh, (int)wpr);
+        if ((st = mk_launch_status("kv4_append")) != MK_OK || fresh) return st;
     }
     hipLaunchKernelGGL(kv4_advance_kernel, dim3((unsigned)((c->B + 255) / 256)), dim3(256), 0, (hipStream_t)stream, v, s, fresh);
     return mk_launch_status("kv4_advance");
@@ -140,8 +181,6 @@ extern "C" int mk_dev_kv4_to_f32(const mk_kv4_cache *c, size_t n, float *k, floa
     MK_REQUIRE(n <= c->cap, "more positions than the cache holds");
     if (n == 0) return MK_OK;
     MK_REQUIRE(k && v && mk_aligned16(k) && mk_aligned16(v), "outputs must be 16-byte aligned");
-    const size_t items = (c->dk + c->rope + c->dv) / 8, total = c->B * n * c->nkv * items;
-    MK_REQUIRE((total + 255) / 256 <= 0x7FFFFFFFull, "too many values in one call");
-    hipLaunchKernelGGL(kv4_to_f32_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, mk_kv4_view(c), (int)n, k, v, (int)items, total);
+    hipLaunchKernelGGL(kv4_to_f32_kernel, dim3((unsigned)((n + SNAP - 1) / SNAP), (unsigned)c->B), dim3(256), 0, (hipStream_t)stream, mk_kv4_view(c), (int)n, k, v);
     return mk_launch_status("kv4_to_f32");
 }

@@ -174,6 +174,33 @@ def test_kv4_store_and_snapshot(nkv, dk, rope, dv, dtype):
     assert not host(gk[0]).any() and not host(gk[1, 17]).any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_kv4_levels_at_and_beside_every_midpoint(dtype):
+    """Rounding is exact arithmetic: the values held equal the definition's, signs of zeros included."""
+    from microkimi_amd import mixer
+    mids = np.array([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32)
+    near = np.concatenate([mids, mids * np.float32(1 - 2.0 ** -8), mids * np.float32(1 + 2.0 ** -7), np.nextafter(mids, np.float32(0)), np.nextafter(mids, np.float32(9))])
+    special = np.array([0.0, -0.0, np.nan, 1e-40, -1e-40, 0.2, -0.2], np.float32)
+    vals = np.concatenate([near, -near, special])
+    vals = np.concatenate([vals, np.zeros(-len(vals) % 31, np.float32)]).reshape(-1, 31)
+    blocks = []
+    for top in (6.0, 4.5, 4.0, 3.2):      # a block's largest value sets its exponent
+        for ex in (-120, -30, -1, 0, 1, 40, 124):
+            b = np.concatenate([np.minimum(np.abs(vals), np.float32(top)) * np.copysign(1, vals), np.full((len(vals), 1), top, np.float32)], 1).astype(np.float32)
+            blocks.append(np.ldexp(b, ex).astype(np.float32))
+    blocks += [np.where(np.arange(32) % 5 == 0, np.float32(x), b).astype(np.float32) for b in blocks[:2] for x in (np.inf, -np.inf, 3e38, -3e38)]
+    x = np.concatenate(blocks)
+    if dtype == "bf16":
+        x = ref.bf16(x).astype(np.float32)
+    n = len(x)
+    c = mixer.KvCache4(1, 1, 32, 32, n)
+    c.push(to_dev(x[:, None], dtype), to_dev(-x[:, None], dtype))
+    k, v = c.to_f32()
+    for got, src in ((host(k[0, :, 0]), x), (host(v[0, :, 0]), -x)):
+        want = ref.mxfp4(src).astype(np.float32)
+        assert np.array_equal(got, want) and np.array_equal(np.signbit(got), np.signbit(want))
+
+
 def test_kv4_rows_beyond_the_capacity_and_behind_the_last_sequence():
     from microkimi_amd import mixer
     torch = torch_cuda()
