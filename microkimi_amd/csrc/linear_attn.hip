@@ -282,17 +282,14 @@ template <int LD> __device__ __forceinline__ mk_f8v column8(const float *tile, i
 
 template <int N> struct Int { static constexpr int value = N; };
 
+// A sequence is cut into segments of `per` blocks, each a slot of the workspace and a workgroup per head; sequence b has the slots from
+// at(b) / (64 per) + b on: never fewer than its segments (some stay empty), T / (64 per) + B in all, whatever the lengths are.
 struct LinSeg {
-    int n_seg;
-    mk_f4 *local;   // [b][h][segment][DK / 16][threads]: local states, then the states before each segment
-    float *decay;   // [b][h][segment]: e^{sum of the segment's log decays}
+    int per;        // 0: a sequence is one workgroup per head, without a workspace
+    mk_f4 *local;   // [slot][h][DK / 16][4 DV]: local states, then the states before each segment
+    float *decay;   // [slot][h]: e^{sum of the segment's log decays}
+    __device__ __forceinline__ int first(const LinArgs &a, int b) const { return a.at(b) / (CH * per) + b; }
 };
-// blocks of segment seg of a sequence with n tokens
-__device__ __forceinline__ void segment(int n, int n_seg, int seg, int &c0, int &c1) {
-    const int nch = (n + CH - 1) / CH, per = (nch + n_seg - 1) / n_seg;
-    c0 = min(seg * per, nch);
-    c1 = min(c0 + per, nch);
-}
 // 2^x for the decays: x is a difference of 64-bit sums of log2 decays, rounded once
 __device__ __forceinline__ float pow2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
@@ -335,14 +332,23 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
     __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
     __shared__ int bad_l;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int h = blockIdx.x % a.nh, seg = blockIdx.x / a.nh % sg.n_seg, b = blockIdx.x / a.nh / sg.n_seg, hk = h / (a.nh / a.nkh);
-    const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0);
-    int c0, c1;
-    segment(len, sg.n_seg, seg, c0, c1);
-    const size_t bh = (size_t)b * a.nh + h, sbase = bh * DK * DV + 16 * NT * wave + n;
-    if (c0 >= c1 && sg.n_seg > 1) return;
+    const int h = blockIdx.x % a.nh, slot = blockIdx.x / a.nh, hk = h / (a.nh / a.nkh);
+    int b = slot, c0 = 0;
+    if (MODE != BOTH) {  // the last sequence whose slots begin at this one or before
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sg.first(a, mid) <= slot) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        c0 = max(slot - sg.first(a, b), 0) * sg.per;
+    }
+    const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0), nch = (len + CH - 1) / CH, c1 = MODE == BOTH ? nch : min(c0 + sg.per, nch);
+    if (MODE != BOTH && c0 >= c1) return;
+    const size_t sh = (size_t)slot * a.nh + h, sbase = ((size_t)b * a.nh + h) * DK * DV + 16 * NT * wave + n;
     mk_f4 S[KT][NT];
-    mk_f4 *mine = sg.local + ((bh * sg.n_seg + seg) * KT) * (DV * 4) + 64 * NT * wave + lane;
+    mk_f4 *mine = sg.local + sh * KT * (DV * 4) + 64 * NT * wave + lane;
 #pragma unroll
     for (int kt = 0; kt < KT; kt++)
 #pragma unroll
@@ -577,7 +583,7 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
                 mine[kt * (DV * 4) + 64 * t] = S[kt][t];
             }
         }
-    if (MODE == LOCAL && threadIdx.x == TH - 1) sg.decay[bh * sg.n_seg + seg] = pow2(total);
+    if (MODE == LOCAL && threadIdx.x == TH - 1) sg.decay[sh] = pow2(total);
 }
 
 // Between the two passes over the segments: local states -> the states before each segment, and the state behind the last.  One
@@ -593,18 +599,20 @@ __global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg 
 #pragma unroll
         for (int j = 0; j < 4; j++) S[j] = a.state[at + (size_t)j * DV];
     }
-    mk_f4 *p = sg.local + (bh * sg.n_seg * KT + kt) * TH + threadIdx.x;
-    const int nch = (len + CH - 1) / CH, per = (nch + sg.n_seg - 1) / sg.n_seg, used = per ? (nch + per - 1) / per : 0;  // (segment())
+    const size_t sh = (size_t)sg.first(a, b) * a.nh + h, step = (size_t)a.nh * KT * TH;
+    mk_f4 *p = sg.local + (sh * KT + kt) * TH + threadIdx.x;
+    const float *decay = sg.decay + sh;
+    const int used = (len + CH * sg.per - 1) / (CH * sg.per);
     for (int s0 = 0; s0 < used; s0 += 8) {
         mk_f4 L[8];
         float E[8];
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (s0 + i < used) L[i] = p[(size_t)(s0 + i) * KT * TH], E[i] = sg.decay[bh * sg.n_seg + s0 + i];
+            if (s0 + i < used) L[i] = p[(s0 + i) * step], E[i] = decay[(size_t)(s0 + i) * a.nh];
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (s0 + i < used) {
-                p[(size_t)(s0 + i) * KT * TH] = S;
+                p[(s0 + i) * step] = S;
 #pragma unroll
                 for (int j = 0; j < 4; j++) S[j] = fmaf(E[i], S[j], L[i][j]);
             }
@@ -613,23 +621,26 @@ __global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg 
     for (int j = 0; j < 4; j++) a.state_out[at + (size_t)j * DV] = S[j];
 }
 
-// Segments that a sequence is cut into: without them a (sequence, head) is one workgroup; with them the keys and values are read
-// twice (local states first, then the outputs from the right states).  As many as fill the device: 2 workgroups a compute unit.
-constexpr int MAX_SEG = 32;
-int segments(size_t T, size_t B, size_t nh) {
-    const size_t blocks = (T / B + CH - 1) / CH, heads = B * nh;
-    size_t n = 512 / heads;
-    n = n < blocks / 2 ? n : blocks / 2;
-    n = n < MAX_SEG ? n : MAX_SEG;
-    return n < 2 ? 1 : (int)n;
+// Blocks of a segment, 0: no segments.  Without them a (sequence, head) is one workgroup; with them the keys and values are read twice
+// (local states first, then the outputs from the right states), and a long sequence beside short ones spreads over the device.
+// As many as two workgroups a compute unit ask for: 8192 tokens of 32 heads 118 us, as 768 or 1024 workgroups 132 and 136 us.
+// Equal lengths (no cu) are better off without from 192 heads on (bfloat16, 128 x 128; without / with): 192 heads of 400 tokens 43 / 64 us, of 1500
+// tokens 135 / 162 us; 128 heads of 400 tokens 41 / 48 us, of 1500 tokens 125 / 90 us.  What cu holds is not known here: up to 256 heads it
+// is taken for ragged (8 sequences of 24 heads, 1 .. 6000 tokens long: 340 / 125 us).
+int segment_blocks(size_t T, size_t B, size_t nh, bool ragged) {
+    const size_t blocks = (T + CH - 1) / CH;
+    if (B * nh > (ragged ? 256 : 191) || blocks < 4 * B) return 0;
+    const size_t per = (blocks * nh + 511) / 512;
+    return (int)(per < 2 ? 2 : per);
 }
+size_t slots(size_t T, size_t B, int per) { return T / ((size_t)CH * per) + B; }
 bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv == 64 || dv == 128); }
 
 template <typename T, int DK, int DV>
 int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
-    const dim3 grid((unsigned)((size_t)a.nh * sg.n_seg * a.B));
+    const dim3 grid((unsigned)(a.nh * (sg.per ? slots(a.T, a.B, sg.per) : (size_t)a.B)));
     int e;
-    if (sg.n_seg == 1) {
+    if (sg.per == 0) {
         hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, BOTH>), grid, dim3(DV * 4 / tiles<T, DK, DV, BOTH>()), 0, st, a, sg);
         return mk_launch_status("linear_block");
     }
@@ -664,8 +675,9 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
 
 extern "C" size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv) {
     if (!B || !nh || !block_widths(dk, dv)) return 256;
-    const size_t n = (size_t)segments(T, B, nh);
-    return n == 1 ? 256 : B * nh * n * dk * dv * 4 + mk_align_up(B * nh * n * 4, 256);
+    const int per = segment_blocks(T, B, nh, true);
+    const size_t n = per ? slots(T, B, per) * nh : 0;
+    return n ? n * dk * dv * 4 + mk_align_up(n * 4, 256) : 256;
 }
 
 extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
@@ -678,9 +690,10 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out};
     hipStream_t hs = (hipStream_t)stream;
     if (!block_widths(dk, dv)) return dtype == MK_F32 ? launch_token<float>(a, hs) : launch_token<__bf16>(a, hs);
-    LinSeg sg{segments(T, B, nh), (mk_f4 *)workspace, nullptr};
-    sg.decay = (float *)((uint8_t *)workspace + B * nh * sg.n_seg * dk * dv * 4);
-    MK_REQUIRE((size_t)nh * sg.n_seg * B <= 0x7FFFFFFFull, "too many heads and sequences in one call");
+    LinSeg sg{segment_blocks(T, B, nh, cu != nullptr), (mk_f4 *)workspace, nullptr};
+    const size_t n = (sg.per ? slots(T, B, sg.per) : B) * nh;
+    sg.decay = sg.per ? (float *)((uint8_t *)workspace + n * dk * dv * 4) : nullptr;
+    MK_REQUIRE(n <= 0x7FFFFFull, "too many heads and sequences in one call");
     return dtype == MK_F32 ? launch_blocks<float>(a, sg, hs) : launch_blocks<__bf16>(a, sg, hs);
 }
 

@@ -397,6 +397,12 @@ def test_linear_long_prompts_and_decays(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[0, 300, 1, 1000, 257, 0], [1279, 1], [128, 1664, 128, 0, 0], [5, 2000, 3, 173, 2]])
+def test_linear_long_and_short_prompts_side_by_side(lens, dtype):
+    check_linear(lens, 2, 1, 64, 64, dtype, seed=len(lens), tail_rows=2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64), (40, 72)])
 def test_linear_values_that_are_not_finite_reach_later_tokens_only(dk, dv, dtype):
     from microkimi_amd import mixer
