@@ -158,19 +158,24 @@ __device__ __forceinline__ mk_b8 fp4x8(uint32_t w, float sc) {
     return mk_b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// The columns of a workgroup: number `idx` in the list of tiles of CT columns of all sequences (a sequence with m rows and group G has
-// m * G columns).  Every wave finds it for itself.  false: past the end of the list.
-__device__ __forceinline__ bool find_tile(const MkSeqs &s, int G, int CT, int idx, int &b, int &tile) {
-    if (!s.cu) {
-        const int per = (s.T / s.B * G + CT - 1) / CT;
-        b = idx / per;
-        tile = idx - b * per;
-        return b < s.B;
+// The work of a workgroup: number `idx` in the list of (tile of CT columns, chunk of the context) of all sequences (a sequence with m rows
+// and group G has m * G columns, and the chunks that its positions fill: what is not there takes no place in the list, so that the
+// workgroups without work come last: between the others they took a third of the time of 32 ragged sequences).  Every wave finds it for itself.  false: past the end of the list.
+__device__ __forceinline__ bool find_work(const MkKv4 &c, const MkSeqs &s, const AttnArgs &a, int G, int CT, int idx, int &b, int &tile, int &split) {
+    if (s.B == 1) {
+        b = 0;
+        tile = idx / a.n_splits;
+        split = idx - tile * a.n_splits;
+        return tile < ((s.at(1) - s.at(0)) * G + CT - 1) / CT;
     }
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < s.B; b0 += 64) {
         const int mine = b0 + lane;
-        int n = mine < s.B ? (max(s.at(mine + 1) - s.at(mine), 0) * G + CT - 1) / CT : 0;
+        int chunks = 1, n = 0;
+        if (mine < s.B) {
+            if (a.n_splits > 1) chunks = min((int)((min(max(c.lens[mine], 0), c.cap) + (int64_t)a.chunk - 1) / a.chunk), a.n_splits);
+            n = (max(s.at(mine + 1) - s.at(mine), 0) * G + CT - 1) / CT * chunks;
+        }
         int sum = n;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -179,10 +184,12 @@ __device__ __forceinline__ bool find_tile(const MkSeqs &s, int G, int CT, int id
         }
         const int total = __shfl(sum, 63, MK_WAVE);
         if (idx < total) {
-            const uint64_t hit = __ballot(sum > idx);
-            const int l = __builtin_ctzll(hit);
+            const int l = __builtin_ctzll(__ballot(sum > idx));
             b = b0 + l;
-            tile = idx - __shfl(sum - n, l, MK_WAVE);
+            const int r = idx - __shfl(sum - n, l, MK_WAVE);
+            chunks = __shfl(chunks, l, MK_WAVE);
+            tile = r / chunks;
+            split = r - tile * chunks;
             return true;
         }
         idx -= total;
@@ -342,11 +349,12 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
     constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::P, LD = DV + 4;
     __shared__ float o_l[4][16][LD], m_l[4][16], l_l[4][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % c.nkv, split = blockIdx.x / c.nkv % a.n_splits, G = a.nh / c.nkv;
-    int b, tile;
-    if (!find_tile(s, G, 16, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
+    const int hk = blockIdx.x % c.nkv, G = a.nh / c.nkv;
+    int b, tile, split;
+    if (!find_work(c, s, a, G, 16, blockIdx.x / c.nkv, b, tile, split)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
+    split = __builtin_amdgcn_readfirstlane(split);
     const Column col = column(c, s, G, hk, b, tile * 16 + n);
     const int top = __builtin_amdgcn_readfirstlane(columns_max(col.lim));
     const int low = __builtin_amdgcn_readfirstlane(columns_min(col.live ? col.lim : 0x7FFFFFFF));
@@ -569,11 +577,12 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : sizeof(T) == 4 ? 2 : 3) void k
     constexpr int NS = DK / 32, NR = R / 32, NF = NS + NR, NK = 2 * NF, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM;
     __shared__ mk_b8 k_l[2][2][NF][64], v_l[2][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % c.nkv, split = blockIdx.x / c.nkv % a.n_splits, G = a.nh / c.nkv;
-    int b, tile;
-    if (!find_tile(s, G, 64, blockIdx.x / c.nkv / a.n_splits, b, tile)) return;
+    const int hk = blockIdx.x % c.nkv, G = a.nh / c.nkv;
+    int b, tile, split;
+    if (!find_work(c, s, a, G, 64, blockIdx.x / c.nkv, b, tile, split)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
+    split = __builtin_amdgcn_readfirstlane(split);
     const Column col = column(c, s, G, hk, b, tile * 64 + wave * 16 + n);
     const int low = __builtin_amdgcn_readfirstlane(columns_min(col.live ? col.lim : 0x7FFFFFFF));
     // the last position that a column of the workgroup sees (limits grow with the column; one beyond the capacity sees nothing)
@@ -758,7 +767,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnA
 
 // Positions of a chunk, when `pairs` (column tile, kv head) walk `len` positions each.  About 1024 chunks fill the 256 compute units; below
 // 256 positions (two steps a wave) a chunk is start and end only, above 1024 one long sequence among short ones is a tail (32
-// ragged sequences: 38.6 / 35.4 / 41.1 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
+// ragged sequences of up to 16384 positions: 30.2 / 24.2 / 27.0 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
 // costs what the split saves (96 heads, 1024 positions: 13.2 us, in four chunks 10.3 + 4.0 us).
 // Many columns: a chunk's result is as large as its columns and the work is bound by the matrix cores, so a context is cut only while
 // the workgroups are fewer than the compute units (512 rows at 4096 positions, 96 heads: four chunks and their merge cost 32 us).

@@ -286,6 +286,14 @@ def test_kv4_long_contexts(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_kv4_many_sequences_of_every_length(dtype):
+    lens = [[0, 1, 40, 1030, 7, 0, 300][i % 7] for i in range(69)] + [2590]
+    check_attn(lens, [min(n, 1) for n in lens], 4, 2, 64, 0, 64, dtype, seed=12)
+    check_attn(lens, [1] * 70, 2, 2, 64, 64, 64, dtype, seed=13, uniform=True, max_len=1500)   # (a hint that is too small)
+    check_attn([1300, 0, 1100, 64], [70, 0, 3, 64], 2, 2, 128, 0, 128, dtype, seed=14, cap=4096)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_kv4_sharp_scores(dtype):
     check_attn([700], [1], 4, 2, 128, 0, 128, dtype, seed=9, sharp=30.0, uniform=True)
     check_attn([90], [33], 4, 2, 128, 64, 128, dtype, seed=10, sharp=30.0)
