@@ -74,7 +74,7 @@ def _f32(ref, t, name, shape=None):
 def _result(out, ref, shape, name, dtype=None):
     """The caller's output tensor after its checks, or a new one."""
     if out is None:
-        return torch.empty(shape, dtype=dtype or ref.dtype, device=ref.device)
+        return ref.new_empty(shape) if dtype is None else ref.new_empty(shape, dtype=dtype)
     _same(ref, out, name, dtype)
     if out.shape != shape or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"{name} must be a contiguous, 16-byte aligned {tuple(shape)} tensor")
@@ -82,6 +82,8 @@ def _result(out, ref, shape, name, dtype=None):
 
 
 def _cu_ptr(ref, cu, B, T):
+    if B < 1:
+        raise ValueError("there must be a sequence")
     if cu is None:
         if T % B:
             raise ValueError(f"{T} rows do not divide among {B} sequences: give cu")

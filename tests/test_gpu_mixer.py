@@ -531,3 +531,14 @@ def test_calls_on_two_streams_at_once():
     for i in range(2):
         for triple in got[i]:
             assert all(torch.equal(x, y) for x, y in zip(triple, want[i]))
+
+
+def test_a_call_without_sequences_is_refused():
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    x, g = torch.zeros((4, 2, 64), device="cuda"), torch.zeros((4, 2), device="cuda")
+    for kw in (dict(B=0), dict(B=-1), dict(cu=ints([0]))):
+        with pytest.raises(ValueError, match="sequence"):
+            mixer.linear_attn(x, x, x, g, **kw)
+    with pytest.raises(ValueError):
+        mixer.KvCache4(0, 1, 32, 32, 4)
