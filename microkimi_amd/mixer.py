@@ -82,8 +82,6 @@ def _result(out, ref, shape, name, dtype=None):
 
 
 def _cu_ptr(ref, cu, B, T):
-    if B < 1:
-        raise ValueError("there must be a sequence")
     if cu is None:
         if T % B:
             raise ValueError(f"{T} rows do not divide among {B} sequences: give cu")
@@ -285,6 +283,8 @@ def linear_attn(q, k, v, g, state=None, scale=1.0, cu=None, B=None, out=None, st
     Returns (out [T, nh, dv], state_out); state_out=state updates in place."""
     if B is None:
         B = cu.shape[0] - 1 if cu is not None else state.shape[0] if state is not None else 1
+    if B < 1:
+        raise ValueError("there must be a sequence")
     dt, q, qs, k, ks, v, vs, g, gs, T, nh, nkh, dk, dv, state, state_out, out = _linear_args(q, k, v, g, state, B, out, state_out)
     cup = _cu_ptr(q, cu, B, T)
     ws = torch.empty(lib.mk_linear_attn_workspace_bytes(T, B, nh, dk, dv), dtype=torch.uint8, device=q.device)
