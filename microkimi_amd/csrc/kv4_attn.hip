@@ -187,10 +187,10 @@ __device__ __forceinline__ bool find_work(const MkKv4 &c, const MkSeqs &s, const
             const int l = __builtin_ctzll(__ballot(sum > idx));
             b = b0 + l;
             const int r = idx - __shfl(sum - n, l, MK_WAVE);
-            chunks = __shfl(chunks, l, MK_WAVE);
+            chunks = max(__shfl(chunks, l, MK_WAVE), 1);
             tile = r / chunks;
             split = r - tile * chunks;
-            return true;
+            return r >= 0 && r < __shfl(n, l, MK_WAVE);  // (sequences that overlap, which no cu should say, may pass 31 bits together)
         }
         idx -= total;
     }
@@ -839,7 +839,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     MK_REQUIRE(q_stride % 8 == 0 && mk_aligned16(q) && mk_aligned16(out) && ((uintptr_t)workspace & 255) == 0,
                "q and out must be 16-byte, the workspace 256-byte aligned, the query stride a multiple of 8 values");
     MK_REQUIRE(T == 1 || q_stride >= nh * (c->dk + c->rope), "the query stride is shorter than a token's heads");
-    MK_REQUIRE(T * nh <= 0x7FFFFFFFull, "too many query rows in one call");
+    MK_REQUIRE(T * nh <= 0x7FFFFF00ull, "too many query rows in one call");
     AttnArgs a;
     a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
@@ -847,6 +847,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     const int ct = columns_of(c, T, group);
     const size_t tiles = matrix ? column_tiles(c, T, cu, group, ct) : T * group;
     plan(a, tiles * c->nkv, len, matrix ? ct : 16);
+    MK_REQUIRE(a.n_splits == 1 || (T * nh + 3) / 4 <= MAX_GROUPS, "too many query rows in one call");
     uint8_t *w = (uint8_t *)workspace;
     a.po = (float *)w;
     w += mk_align_up((size_t)a.n_splits * T * nh * c->dv * 4, 256);
@@ -857,7 +858,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     const MkKv4 v = mk_kv4_view(c);
     hipStream_t hs = (hipStream_t)stream;
     if (matrix) {
-        MK_REQUIRE(tiles * c->nkv * a.n_splits <= 0x7FFFFFFFull, "too many query rows in one call");
+        MK_REQUIRE(tiles * c->nkv * a.n_splits <= MAX_GROUPS, "too many query rows in one call");
         const dim3 grid((unsigned)(tiles * c->nkv * a.n_splits));
         if (dtype == MK_F32) launch_matrix<float>(ct, grid, hs, v, s, a);
         else launch_matrix<__bf16>(ct, grid, hs, v, s, a);

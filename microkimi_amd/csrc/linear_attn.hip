@@ -9,7 +9,6 @@
 
 namespace {
 
-
 struct LinArgs {
     const void *q, *k, *v;
     size_t qs, ks, vs;      // values from one token's row to the next
@@ -181,7 +180,6 @@ int launch_token(const LinArgs &a, hipStream_t st) {
     else hipLaunchKernelGGL((linear_token_kernel<T, 16>), grid, dim3(256), 0, st, a);
     return mk_launch_status("linear_token");
 }
-
 
 // ------------------------------------------------------------------------------------------------ blocks of 64 tokens
 //
@@ -693,7 +691,7 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     LinSeg sg{segment_blocks(T, B, nh, cu != nullptr), (mk_f4 *)workspace, nullptr};
     const size_t n = (sg.per ? slots(T, B, sg.per) : B) * nh;
     sg.decay = sg.per ? (float *)((uint8_t *)workspace + n * dk * dv * 4) : nullptr;
-    MK_REQUIRE(n <= 0x7FFFFFull, "too many heads and sequences in one call");
+    MK_REQUIRE(n <= MAX_GROUPS / 2, "too many heads and sequences in one call");
     return dtype == MK_F32 ? launch_blocks<float>(a, sg, hs) : launch_blocks<__bf16>(a, sg, hs);
 }
 

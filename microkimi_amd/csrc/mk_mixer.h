@@ -5,6 +5,8 @@
 typedef __bf16 mk_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 mk_b2 __attribute__((ext_vector_type(2)));
 
+constexpr size_t MAX_GROUPS = 0xFFFFFF;  // workgroups of 256 threads in one dimension of a grid, which has 2^32 threads
+
 static inline size_t mk_align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 static inline bool mk_aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 

@@ -143,13 +143,13 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
 template <typename T, int LPR>
 int launch(NormRopeArgs a, size_t n_tok, int halves, hipStream_t st) {
     constexpr int GROUPS = 256 / LPR;
-    // From 1024 tokens on a token is one workgroup (its heads share the table's row and the weights, the device is full: 8192 tokens of 64 + 8
-    // bfloat16 heads of 128 62 us, one head a group of lanes 77 us); below, every group of lanes gets one head (777 tokens of 96 + 96
-    // f32 heads of 192: 45 us, as one workgroup a token 55 us).
+    // From 1024 tokens on a token is one workgroup: its heads share the table's row and the weights, and the device is full (8192 tokens of
+    // 64 + 8 bfloat16 heads of 128: 62 us, with one head a group of lanes 77 us).  Below, every group of lanes gets one head (777
+    // tokens of 96 + 96 f32 heads of 192: 52 us, as one workgroup a token 59 us).
     a.apart = n_tok < 1024;
     a.parts = a.apart ? ((a.nh > a.nkv ? a.nh : a.nkv) + GROUPS - 1) / GROUPS : 1;
     const size_t grid = n_tok * (size_t)a.parts * (a.apart ? 2 : 1);
-    MK_REQUIRE(grid <= 0x7FFFFFFFull, "too many rows in one call");
+    MK_REQUIRE(grid <= MAX_GROUPS, "too many rows in one call");
     if (halves)
         hipLaunchKernelGGL((norm_rope_kernel<T, LPR, true>), dim3((unsigned)grid), dim3(256), 0, st, a);
     else
@@ -164,7 +164,6 @@ int launch_width(const NormRopeArgs &a, size_t n_tok, int halves, hipStream_t st
     if (a.hd <= 256) return launch<T, 32>(a, n_tok, halves, st);
     return launch<T, 64>(a, n_tok, halves, st);
 }
-
 
 }  // namespace
 
