@@ -124,8 +124,11 @@ __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, At
 // position, which is one block (one scale byte) at DK = 128.
 //
 // 4-bit values become bfloat16 exactly (two significant bits, and the exponent of an f32), so the products are exact in f32.
-// f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as PT terms: three
-// for f32 results, two (17 bits) for bfloat16 results, whose own rounding is 2^-8.
+// f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as P terms (few
+// columns) or PM terms (many): three for f32 results.  For bfloat16 results, whose own rounding is up to 2^-9, two (17 bits) where the
+// product costs no time (few columns are bound by memory: one term 59.7, two 59.8 us at 96 heads x 16384 positions), and one where it
+// does (512 rows behind 3584 positions: one term 160, two 192 us): its roundings, 2^-9 of each weight, are as large as the result's
+// at most and average out over the positions.
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float FAR = 1048576.0f;  // 2^20: weights up to this above the reference point are summed as they are
 
@@ -242,6 +245,10 @@ __device__ __forceinline__ void load_query(const AttnArgs &a, const Column &o, i
 }
 
 // ------------------------------------------------------------------------- few query columns: every wave its own positions
+//
+// Bound by memory: 96 heads over 16384 positions of 128 + 64 | 128, bfloat16 queries (216 MB): 48 us, 4.5 TB/s, and 4.8 us for the merge; 32
+// sequences of 1 .. 16384 positions, 8 kv heads (99.7 MB) 24.4 + 4.4 us; 1024 positions of 96 heads 12.6 us, the rate of 96 compute
+// units (eight waves instead of four: 11.6 us for 10.6).
 //
 // One workgroup: (tile of 16 query columns, kv head, chunk of the context), the heads fastest: neighbours in the grid, which go to
 // the eight XCDs in turn, then have the same length (with the sequences fastest a long one's workgroups all met on one XCD:
@@ -487,6 +494,10 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(Mk
 }
 
 // ----------------------------------------------------------------------- many query columns: the workgroup shares K and V
+//
+// 512 rows behind 3584 positions, 96 heads of 128 + 64 | 128 in bfloat16 (121 GFLOP): 160 us, 756 TFLOP/s (a large library product:
+// 1085).  Operand reads from LDS (80 KB a step and workgroup) alone take 96 us, vector issue 72, the matrix cores 49; without the fetches
+// it is 141 us.  32 columns a wave would halve the reads, but 128 columns a workgroup leave 384 of them to 512 places.
 //
 // One workgroup: (tile of 64 query columns, 16 a wave; kv head; chunk of the context), 32 positions a step.  Waves 0 and 1 turn the K
 // rows of 16 positions each into bfloat16 operands in LDS, waves 2 and 3 the V rows (as in the kernel above, so no transposed read
@@ -769,7 +780,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnA
 // 256 positions (two steps a wave) a chunk is start and end only, above 1024 one long sequence among short ones is a tail (32
 // ragged sequences of up to 16384 positions: 30.2 / 24.2 / 27.0 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
 // costs what the split saves (96 heads, 1024 positions: 13.2 us, in four chunks 10.3 + 4.0 us).
-// Many columns: a chunk's result is as large as its columns and the work is bound by the matrix cores, so a context is cut only while
+// Many columns: a chunk's result is as large as its columns and the work is not bound by memory, so a context is cut only while
 // the workgroups are fewer than the compute units (512 rows at 4096 positions, 96 heads: four chunks and their merge cost 32 us).
 void plan(AttnArgs &a, size_t pairs, size_t len, int ct) {
     size_t chunk = (pairs * len / (ct > 16 ? 512 : 1024) + 127) / 128 * 128;
