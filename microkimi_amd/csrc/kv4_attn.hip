@@ -4,7 +4,6 @@
 namespace {
 
 constexpr int MAX_SPLITS = 64;
-constexpr int MAX_CT = 64;  // the most query columns that a workgroup of any form below takes
 
 // --------------------------------------------------------------------------------------------------- attention: any width
 
@@ -352,7 +351,7 @@ template <int DV> struct VStep {
 };
 
 template <typename T, int DK, int R, int DV>
-__global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv4_attn_few_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+__global__ __launch_bounds__(256, DK == 256 && sizeof(T) == 4 ? 1 : 2) void kv4_attn_few_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
     constexpr int NS = DK / 32, NR = R / 32, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::P, LD = DV + 4;
     __shared__ float o_l[4][16][LD], m_l[4][16], l_l[4][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -583,8 +582,12 @@ template <typename T, int N> __device__ __forceinline__ void store_run(void *out
     }
 }
 
+// Workgroups of the kernel below that a compute unit holds (registers; at width 256 two instead of one: 512 rows at 4096 positions, 16 heads,
+// 73 us instead of 113).
+constexpr int many_per_cu(size_t elem, size_t dk) { return dk == 256 ? (elem == 4 ? 1 : 2) : elem == 4 ? 2 : 3; }
+
 template <typename T, int DK, int R, int DV>
-__global__ __launch_bounds__(256, DK == 256 ? 1 : sizeof(T) == 4 ? 2 : 3) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
+__global__ __launch_bounds__(256, many_per_cu(sizeof(T), DK)) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
     constexpr int NS = DK / 32, NR = R / 32, NF = NS + NR, NK = 2 * NF, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM;
     __shared__ mk_b8 k_l[2][2][NF][64], v_l[2][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -776,24 +779,39 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(MkKv4 c, MkSeqs s, AttnA
     }
 }
 
-// Positions of a chunk, when `pairs` (column tile, kv head) walk `len` positions each.  About 1024 chunks fill the 256 compute units; below
-// 256 positions (two steps a wave) a chunk is start and end only, above 1024 one long sequence among short ones is a tail (32
-// ragged sequences of up to 16384 positions: 30.2 / 24.2 / 27.0 us in chunks of 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch
-// costs what the split saves (96 heads, 1024 positions: 13.2 us, in four chunks 10.3 + 4.0 us).
-// Many columns: a chunk's result is as large as its columns and the work is not bound by memory, so a context is cut only while
-// the workgroups are fewer than the compute units (512 rows at 4096 positions, 96 heads: four chunks and their merge cost 32 us).
-void plan(AttnArgs &a, size_t pairs, size_t len, int ct) {
-    size_t chunk = (pairs * len / (ct > 16 ? 512 : 1024) + 127) / 128 * 128;
-    if (ct > 16) chunk = len <= 1024 || pairs >= 256 ? len : chunk < 256 ? 256 : chunk;
-    else chunk = len <= 1024 ? len : chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+// Prompts of widths that have no matrix kernel: enough workgroups without a cut, whose results would be as large as the rows.
+bool uncut(int columns, size_t T, size_t B, size_t pairs) { return columns == 1 && T > B && pairs >= 1024; }
+
+// the widths the matrix kernels are built for: (K, tail, V)
+bool matrix_widths(const mk_kv4_cache *c) {
+    return c->dk == c->dv ? (c->dk == 64 || c->dk == 128 || c->dk == 256) && (c->rope == 0 || c->rope == 64) : false;
+}
+
+// Which kernel a call takes, by the query columns a sequence has on average: a wave's 16 are all there is, or the workgroup shares K and V.
+// (The kernel for 16 reads 32 positions at a time and a cache has to hold them; the other reads none past the last.)
+enum Form { FEW = 16, MANY = 64, ANY = 1 };  // the value: query columns of a workgroup
+Form form_of(const mk_kv4_cache *c, size_t T, size_t group) {
+    if (!matrix_widths(c)) return ANY;
+    return T * group <= FEW * c->B && c->cap >= 32 ? FEW : MANY;
+}
+
+// Chunks that a context is cut into when `pairs` (column tile, kv head) walk `len` positions each.
+//
+// Few columns: about 1024 chunks fill the 256 compute units; below 256 positions (two steps a wave) a chunk is start and end only,
+// above 1024 one long sequence among short ones is a tail (32 ragged sequences of up to 16384 positions: 30.2 / 24.2 / 27.0 us in chunks of
+// 512 / 1024 / 2048).  Up to 1024 positions are one chunk: the second launch costs what the split saves (96 heads, 1024
+// positions: 13.2 us, in four chunks 10.3 + 4.0 us).
+void plan_few(AttnArgs &a, size_t pairs, size_t len) {
+    size_t chunk = (pairs * len / 1024 + 127) / 128 * 128;
+    chunk = len <= 1024 ? len : chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
     const size_t least = (len + MAX_SPLITS - 1) / MAX_SPLITS;
-    if (chunk < least && chunk < len) chunk = (least + 127) / 128 * 128;
+    if (chunk < least) chunk = (least + 127) / 128 * 128;
     a.chunk = (int)chunk;
     a.n_splits = (int)((len + chunk - 1) / chunk);
 }
-// The most chunks that plan() makes for `pairs` or more and any length up to cap: chunks of 256 until pairs * len reaches 1024 * 256, then
+// The most chunks that it makes for `pairs` or more and any length up to cap: chunks of 256 until pairs * len reaches 1024 * 256, then
 // at most 1024 / pairs (and one that is not whole) of them, from chunks of 1024 on len / 1024.
-size_t most_splits(size_t pairs, size_t cap) {
+size_t most_few(size_t pairs, size_t cap) {
     if (cap <= 1024) return 1;
     size_t n = (1024 + pairs - 1) / pairs + 1;
     const size_t by_len = (cap + 1023) / 1024;
@@ -802,41 +820,62 @@ size_t most_splits(size_t pairs, size_t cap) {
     return n < MAX_SPLITS ? n : MAX_SPLITS;
 }
 
-// the widths the matrix kernels are built for: (K, tail, V)
-bool matrix_widths(const mk_kv4_cache *c) {
-    return c->dk == c->dv ? (c->dk == 64 || c->dk == 128 || c->dk == 256) && (c->rope == 0 || c->rope == 64) : false;
+// Many columns: the number of chunks with the least estimated time, of those that make no more than about 1024 workgroups.  A step of 32
+// positions takes 0.3 + 0.5 us for every 256 values of K and V (f32: 1.8 times that); a second workgroup on a compute unit costs 5 %, a third
+// 20 % more; a merge takes 8 us and its results' way to memory and back.  (96 heads over 4096 positions: 192 rows 129 us uncut, 103 in two
+// chunks, 300 rows 133 and 165; 200 rows of 48 heads over 16000: 194 us in four chunks, 143 in six.)
+size_t most_many(size_t pairs, size_t cap) {
+    size_t n = (1024 + pairs - 1) / pairs;
+    n = n < cap / 256 ? n : cap / 256;
+    n = n < MAX_SPLITS ? n : MAX_SPLITS;
+    return n < 1 ? 1 : n;
 }
+void plan_many(AttnArgs &a, size_t pairs, size_t len, size_t rows, size_t elem, const mk_kv4_cache *c) {
+    const size_t at_once = many_per_cu(elem, c->dk);
+    const double share[4] = {0.0, 1.0, 1.05, 1.25};  // time of 0 .. 3 workgroups on a compute unit
+    const double step = (0.3 + 0.5 * (c->dk + c->rope + c->dv) / 256) * (elem == 4 ? 1.8 : 1.0);
+    double best = 0.0;
+    a.chunk = (int)len, a.n_splits = 1;
+    for (size_t n = 1; n <= most_many(pairs, len); n++) {
+        const size_t chunk = n == 1 ? len : ((len + n - 1) / n + 127) / 128 * 128, splits = (len + chunk - 1) / chunk;
+        const size_t on_cu = (pairs * splits + 255) / 256;
+        double t = chunk / 32.0 * step * (on_cu / at_once * share[at_once] + share[on_cu % at_once]);
+        if (splits > 1) t += 8.0 + splits * rows * c->dv * 8 / 3e6;
+        if (n > 1 && t >= best) continue;
+        best = t, a.chunk = (int)chunk, a.n_splits = (int)splits;
+    }
+}
+
 size_t column_tiles(const mk_kv4_cache *c, size_t T, const int32_t *cu, size_t group, size_t ct) {
     return cu ? T * group / ct + c->B : c->B * ((T / c->B * group + ct - 1) / ct);
 }
 
-// ct: query columns of a workgroup (16: every wave its own positions; 64: the workgroup shares K and V)
 template <typename T, int D, int R>
-void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
-    if (ct == 16) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
+void launch_matrix(Form form, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (form == FEW) hipLaunchKernelGGL((kv4_attn_few_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
     else hipLaunchKernelGGL((kv4_attn_many_kernel<T, D, R, D>), grid, dim3(256), 0, st, v, s, a);
 }
 template <typename T, int D>
-void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
-    if (v.rope) launch_matrix<T, D, 64>(ct, grid, st, v, s, a);
-    else launch_matrix<T, D, 0>(ct, grid, st, v, s, a);
+void launch_matrix(Form form, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.rope) launch_matrix<T, D, 64>(form, grid, st, v, s, a);
+    else launch_matrix<T, D, 0>(form, grid, st, v, s, a);
 }
 template <typename T>
-void launch_matrix(int ct, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
-    if (v.dk == 64) launch_matrix<T, 64>(ct, grid, st, v, s, a);
-    else if (v.dk == 128) launch_matrix<T, 128>(ct, grid, st, v, s, a);
-    else launch_matrix<T, 256>(ct, grid, st, v, s, a);
+void launch_matrix(Form form, const dim3 &grid, hipStream_t st, const MkKv4 &v, const MkSeqs &s, const AttnArgs &a) {
+    if (v.dk == 64) launch_matrix<T, 64>(form, grid, st, v, s, a);
+    else if (v.dk == 128) launch_matrix<T, 128>(form, grid, st, v, s, a);
+    else launch_matrix<T, 256>(form, grid, st, v, s, a);
 }
-// Query columns of a workgroup, by the columns a sequence has on average: a wave's 16 are all there is, or the workgroup shares K and V.
-int columns_of(const mk_kv4_cache *c, size_t T, size_t group) { return T * group <= 16 * c->B ? 16 : 64; }
 
 }  // namespace
 
 extern "C" size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh) {
     if (!c || !T || !nh || !c->nkv || !c->cap) return 256;
-    // no form of the call has fewer (column tile, kv head) pairs than this
-    const size_t cols = T * (nh / c->nkv ? nh / c->nkv : 1), pairs = c->nkv * (cols / MAX_CT ? cols / MAX_CT : 1);
-    const size_t n = most_splits(pairs, c->cap);
+    // (column tile, kv head) pairs: no fewer than this, wherever the sequences begin
+    const size_t group = nh / c->nkv ? nh / c->nkv : 1, cols = T * group;
+    const Form form = form_of(c, T, group);
+    const size_t pairs = c->nkv * (cols / form ? cols / form : 1);
+    const size_t n = form == MANY ? most_many(pairs, c->cap) : uncut(form, T, c->B, pairs) ? 1 : most_few(pairs, c->cap);
     return n <= 1 ? 256 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
 }
 
@@ -854,10 +893,11 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     AttnArgs a;
     a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
-    const bool matrix = matrix_widths(c) && c->cap >= 32;
-    const int ct = columns_of(c, T, group);
-    const size_t tiles = matrix ? column_tiles(c, T, cu, group, ct) : T * group;
-    plan(a, tiles * c->nkv, len, matrix ? ct : 16);
+    const Form form = form_of(c, T, group);
+    const size_t tiles = form == ANY ? T * group : column_tiles(c, T, cu, group, form), pairs = tiles * c->nkv;
+    if (form == MANY) plan_many(a, pairs, len, T * nh, dtype == MK_F32 ? 4 : 2, c);
+    else if (uncut(form, T, c->B, pairs)) a.chunk = (int)len, a.n_splits = 1;
+    else plan_few(a, pairs, len);
     MK_REQUIRE(a.n_splits == 1 || (T * nh + 3) / 4 <= MAX_GROUPS, "too many query rows in one call");
     uint8_t *w = (uint8_t *)workspace;
     a.po = (float *)w;
@@ -868,11 +908,11 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     const MkSeqs s{cu, (int)T, (int)c->B};
     const MkKv4 v = mk_kv4_view(c);
     hipStream_t hs = (hipStream_t)stream;
-    if (matrix) {
-        MK_REQUIRE(tiles * c->nkv * a.n_splits <= MAX_GROUPS, "too many query rows in one call");
-        const dim3 grid((unsigned)(tiles * c->nkv * a.n_splits));
-        if (dtype == MK_F32) launch_matrix<float>(ct, grid, hs, v, s, a);
-        else launch_matrix<__bf16>(ct, grid, hs, v, s, a);
+    if (form != ANY) {
+        MK_REQUIRE(pairs * a.n_splits <= MAX_GROUPS, "too many query rows in one call");
+        const dim3 grid((unsigned)(pairs * a.n_splits));
+        if (dtype == MK_F32) launch_matrix<float>(form, grid, hs, v, s, a);
+        else launch_matrix<__bf16>(form, grid, hs, v, s, a);
     } else {
         const dim3 grid((unsigned)T, (unsigned)nh, (unsigned)a.n_splits);
         if (dtype == MK_F32) hipLaunchKernelGGL(kv4_attn_any_kernel<float>, grid, dim3(256), 0, hs, v, s, a);
