@@ -294,6 +294,14 @@ def test_kv4_many_sequences_of_every_length(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_kv4_prompts_in_pieces_and_uncut(dtype):
+    check_attn([1500, 40], [20, 3], 16, 2, 256, 0, 256, dtype, seed=15)
+    check_attn([1100], [33], 2, 2, 256, 64, 256, dtype, seed=16)
+    check_attn([1300], [300], 4, 2, 96, 8, 160, dtype, seed=17)      # widths without a matrix kernel: 1200 workgroups, no pieces
+    check_attn([9, 20, 1], [9, 2, 1], 8, 2, 128, 64, 128, dtype, seed=18, cap=20)   # fewer than 32 positions of room
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_kv4_sharp_scores(dtype):
     check_attn([700], [1], 4, 2, 128, 0, 128, dtype, seed=9, sharp=30.0, uniform=True)
     check_attn([90], [33], 4, 2, 128, 64, 128, dtype, seed=10, sharp=30.0)
