@@ -99,52 +99,51 @@ __global__ __launch_bounds__(256) void kv4_advance_kernel(MkKv4 c, MkSeqs s, int
 
 // ------------------------------------------------------------------------------------------------------------ to_f32
 
-// HBM-bound: four sequences of 2048 positions of 8 heads of 128 + 128 (67 MB written) 13.7 us, the rate of a large copy.
-// One workgroup: SNAP positions of a sequence, a thread 4 values at a time (a wave stores 1 KiB in a row); positions a sequence does
-// not hold are zero.
+// A thread: 4 values (an item of a position's K or V rows) of SNAP positions of a sequence, so that a wave stores 1 KiB in a row; positions
+// a sequence does not hold are zero.  HBM-bound: 1500 positions of 96 heads of 192 + 128 (184 MB written) 32 us, 5.8 TB/s (with two and
+// four items a thread 34.5 and 37.4 us); four sequences of 2048 positions of 8 heads of 128 + 128 12.4 us.
 constexpr int SNAP = 4;
 
-__global__ __launch_bounds__(256) void kv4_to_f32_kernel(MkKv4 c, int n, float *__restrict__ k, float *__restrict__ v) {
-    const int b = blockIdx.y, p0 = blockIdx.x * SNAP;
+__global__ __launch_bounds__(256) void kv4_to_f32_kernel(MkKv4 c, int n, int parts, float *__restrict__ k, float *__restrict__ v) {
+    const int b = blockIdx.y, p0 = blockIdx.x / parts * SNAP, item = blockIdx.x % parts * 256 + threadIdx.x;
     const int len = c.lens[b], wk = c.dk + c.rope, nk = c.nkv * wk / 4, nv = c.nkv * c.dv / 4;
-    for (int item = threadIdx.x; item < nk + nv; item += 256) {
-        const bool is_v = item >= nk;
-        const int e = (is_v ? item - nk : item) * 4, across = is_v ? c.dv : wk, h = e / across, d = e - h * across;
-        const bool tail = !is_v && d >= c.dk;
-        const int width = is_v ? c.dv : c.dk;
-        const size_t at = ((size_t)b * c.nkv + h) * c.cap + p0;
-        const uint8_t *codes = (is_v ? c.vq : c.kq) + at * (width / 2) + d / 2, *scales = (is_v ? c.vs : c.ks) + at * (width / 32) + d / 32;
-        float *dst = (is_v ? v : k) + ((size_t)b * n + p0) * c.nkv * across + e;
-        mk_f4 o[SNAP];
-        if (tail) {
-            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    if (item >= nk + nv) return;
+    const bool is_v = item >= nk;
+    const int e = (is_v ? item - nk : item) * 4, across = is_v ? c.dv : wk, h = e / across, d = e - h * across;
+    const bool tail = !is_v && d >= c.dk;
+    const int width = is_v ? c.dv : c.dk;
+    const size_t at = ((size_t)b * c.nkv + h) * c.cap + p0;
+    const uint8_t *codes = (is_v ? c.vq : c.kq) + at * (width / 2) + d / 2, *scales = (is_v ? c.vs : c.ks) + at * (width / 32) + d / 32;
+    float *dst = (is_v ? v : k) + ((size_t)b * n + p0) * c.nkv * across + e;
+    mk_f4 o[SNAP];
+    if (tail) {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int p = 0; p < SNAP; p++) {
-                o[p] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (p0 + p < min(len, n)) {
-                    const b4 x = *(const b4 *)(c.kr + ((size_t)b * c.cap + p0 + p) * c.rope + d - c.dk);
-                    o[p] = mk_f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-                }
+        for (int p = 0; p < SNAP; p++) {
+            o[p] = mk_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p0 + p < min(len, n)) {
+                const b4 x = *(const b4 *)(c.kr + ((size_t)b * c.cap + p0 + p) * c.rope + d - c.dk);
+                o[p] = mk_f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
             }
-        } else {
-            uint32_t code[SNAP], byte[SNAP];
+        }
+    } else {
+        uint32_t code[SNAP], byte[SNAP];
 #pragma unroll
-            for (int p = 0; p < SNAP; p++) {
-                code[p] = byte[p] = 0;
-                if (p0 + p < min(len, n)) code[p] = *(const uint16_t *)(codes + (size_t)p * (width / 2)), byte[p] = scales[(size_t)p * (width / 32)];
-            }
-#pragma unroll
-            for (int p = 0; p < SNAP; p++) {
-                typedef float f2 __attribute__((ext_vector_type(2)));
-                const float sc = mk_scale_from_byte(byte[p]);
-                const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 0), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 1);
-                o[p] = mk_f4{x[0] * sc, x[1] * sc, y[0] * sc, y[1] * sc};
-            }
+        for (int p = 0; p < SNAP; p++) {
+            code[p] = byte[p] = 0;
+            if (p0 + p < min(len, n)) code[p] = *(const uint16_t *)(codes + (size_t)p * (width / 2)), byte[p] = scales[(size_t)p * (width / 32)];
         }
 #pragma unroll
         for (int p = 0; p < SNAP; p++) {
-            if (p0 + p < n) __builtin_nontemporal_store(o[p], (mk_f4 *)(dst + (size_t)p * c.nkv * across));
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            const float sc = mk_scale_from_byte(byte[p]);
+            const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 0), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[p], 1.0f, 1);
+            o[p] = mk_f4{x[0] * sc, x[1] * sc, y[0] * sc, y[1] * sc};
         }
+    }
+#pragma unroll
+    for (int p = 0; p < SNAP; p++) {
+        if (p0 + p < n) __builtin_nontemporal_store(o[p], (mk_f4 *)(dst + (size_t)p * c.nkv * across));
     }
 }
 
@@ -181,6 +180,8 @@ extern "C" int mk_dev_kv4_to_f32(const mk_kv4_cache *c, size_t n, float *k, floa
     MK_REQUIRE(n <= c->cap, "more positions than the cache holds");
     if (n == 0) return MK_OK;
     MK_REQUIRE(k && v && mk_aligned16(k) && mk_aligned16(v), "outputs must be 16-byte aligned");
-    hipLaunchKernelGGL(kv4_to_f32_kernel, dim3((unsigned)((n + SNAP - 1) / SNAP), (unsigned)c->B), dim3(256), 0, (hipStream_t)stream, mk_kv4_view(c), (int)n, k, v);
+    const size_t parts = (c->nkv * (c->dk + c->rope + c->dv) / 4 + 255) / 256, grid = (n + SNAP - 1) / SNAP * parts;
+    MK_REQUIRE(grid <= MAX_GROUPS, "too many values in one call");
+    hipLaunchKernelGGL(kv4_to_f32_kernel, dim3((unsigned)grid, (unsigned)c->B), dim3(256), 0, (hipStream_t)stream, mk_kv4_view(c), (int)n, (int)parts, k, v);
     return mk_launch_status("kv4_to_f32");
 }
