@@ -892,6 +892,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     MK_REQUIRE(T * nh <= 0x7FFFFF00ull, "too many query rows in one call");
     AttnArgs a;
     a.q = q, a.q_stride = q_stride, a.out = out, a.nh = (int)nh, a.scale_log2 = fabsf(scale) * LOG2E, a.sign = scale < 0.0f ? -1.0f : 1.0f;
+    if (scale == 0.0f) a.sign = 0.0f, a.scale_log2 = 1.0f;  // (a hidden position's -inf times 0 would be NaN)
     const size_t len = max_len && max_len < c->cap ? max_len : c->cap, group = nh / c->nkv;
     const Form form = form_of(c, T, group);
     const size_t tiles = form == ANY ? T * group : column_tiles(c, T, cu, group, form), pairs = tiles * c->nkv;

@@ -222,7 +222,7 @@ def test_kv4_rows_beyond_the_capacity_and_behind_the_last_sequence():
     assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all()
 
 
-def check_attn(lens, news, nh, nkv, dk, rope, dv, dtype, seed=0, sharp=1.0, cap=None, uniform=False, strided=False, max_len=None, tail_rows=0):
+def check_attn(lens, news, nh, nkv, dk, rope, dv, dtype, seed=0, sharp=1.0, cap=None, uniform=False, strided=False, max_len=None, tail_rows=0, scale=None):
     """Sequences of lens positions, of which the last news[b] are the rows of the call."""
     from microkimi_amd import mixer
     torch = torch_cuda()
@@ -246,7 +246,7 @@ def check_attn(lens, news, nh, nkv, dk, rope, dv, dtype, seed=0, sharp=1.0, cap=
         wide[:, 1:-1] = q
         q = wide[:, 1:-1]
     out = torch.full((q.shape[0], nh, dv), 7.0, dtype=q.dtype, device="cuda")
-    scale = (dk + rope) ** -0.5
+    scale = (dk + rope) ** -0.5 if scale is None else scale
     got = host(c.attn(q, scale, cu=None if uniform else cu_of(news), out=out, max_len=max_len))
     assert (got[T:] == 7.0).all()
     t, wants = 0, []
@@ -305,6 +305,13 @@ def test_kv4_prompts_in_pieces_and_uncut(dtype):
 def test_kv4_sharp_scores(dtype):
     check_attn([700], [1], 4, 2, 128, 0, 128, dtype, seed=9, sharp=30.0, uniform=True)
     check_attn([90], [33], 4, 2, 128, 64, 128, dtype, seed=10, sharp=30.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,dk,rows_", [(4, 2, 128, 1), (4, 2, 64, 40), (2, 1, 96, 5)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.3, 1e-42])
+def test_kv4_scales_that_are_zero_negative_or_tiny(nh, nkv, dk, rows_, scale, dtype):
+    check_attn([50, 41], [rows_, rows_], nh, nkv, dk, 0, dk, dtype, seed=19, scale=scale)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
