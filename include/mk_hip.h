@@ -468,7 +468,8 @@ int mk_dev_kv4_to_f32(const mk_kv4_cache *c, size_t n, float *k, float *v, void 
  * head h reads kv head h / (nh / nkv).  s_j = scale * q . k_j, out = sum softmax(s)_j v_j.  A row that has no position to
  * attend (an empty sequence) gives zeros, one that would have to attend a position beyond cap gives NaN.
  * max_len: an upper bound of lens, if the caller has one (0: none); it only steers how the work is split.
- * workspace: mk_kv4_attn_workspace_bytes(c, T, nh) bytes, 256-byte aligned, one for each call that may run at the same time. */
+ * workspace: mk_kv4_attn_workspace_bytes(c, T, nh) bytes, 256-byte aligned (0: may be NULL), one for each call that may run at
+ * the same time. */
 size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh);
 int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_stride, size_t T, const int32_t *cu, size_t nh, float scale,
                     size_t max_len, void *workspace, void *out, void *stream);
@@ -479,8 +480,8 @@ int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_st
  * [T] rows of nh at g_stride, or, g_stride == 0, one constant per head [nh]; -inf empties the state.  state [B][nh][dk][dv]
  * (NULL: zeros) is the state before the call, state_out the one after it; they may be the same memory.  A sequence without
  * tokens keeps its state.  dk, dv multiples of 8 up to 256; pointers 16-byte aligned.
- * _attn is the form for prompts (workspace: mk_linear_attn_workspace_bytes, 256-byte aligned, one for each call that may run
- * at the same time), _step the one for a single token of each of B sequences (rows b of q, k, v, g and out). */
+ * _attn is the form for prompts (workspace: mk_linear_attn_workspace_bytes, 256-byte aligned, 0: may be NULL, one for each call that may
+ * run at the same time), _step the one for a single token of each of B sequences (rows b of q, k, v, g and out). */
 size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv);
 int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
                        size_t g_stride, size_t T, const int32_t *cu, size_t B, size_t nh, size_t nkh, size_t dk, size_t dv, float scale,

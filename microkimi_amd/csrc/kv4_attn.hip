@@ -870,13 +870,13 @@ void launch_matrix(Form form, const dim3 &grid, hipStream_t st, const MkKv4 &v, 
 }  // namespace
 
 extern "C" size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh) {
-    if (!c || !T || !nh || !c->nkv || !c->cap) return 256;
+    if (!c || !T || !nh || !c->nkv || !c->cap) return 0;
     // (column tile, kv head) pairs: no fewer than this, wherever the sequences begin
     const size_t group = nh / c->nkv ? nh / c->nkv : 1, cols = T * group;
     const Form form = form_of(c, T, group);
     const size_t pairs = c->nkv * (cols / form ? cols / form : 1);
     const size_t n = form == MANY ? most_many(pairs, c->cap) : uncut(form, T, c->B, pairs) ? 1 : most_few(pairs, c->cap);
-    return n <= 1 ? 256 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
+    return n <= 1 ? 0 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
 }
 
 extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_stride, size_t T, const int32_t *cu, size_t nh, float scale,
@@ -885,7 +885,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     if (st != MK_OK || (st = mk_kv4_check_rows(c, dtype, T, cu)) != MK_OK) return st;
     MK_REQUIRE(nh >= 1 && nh <= 65535 && nh % c->nkv == 0, "the query heads must be a multiple of the kv heads");
     if (T == 0) return MK_OK;
-    MK_REQUIRE(q && out && workspace, "null pointer");
+    MK_REQUIRE(q && out && (workspace || mk_kv4_attn_workspace_bytes(c, T, nh) == 0), "null pointer");
     MK_REQUIRE(q_stride % 8 == 0 && mk_aligned16(q) && mk_aligned16(out) && ((uintptr_t)workspace & 255) == 0,
                "q and out must be 16-byte, the workspace 256-byte aligned, the query stride a multiple of 8 values");
     MK_REQUIRE(T == 1 || q_stride >= nh * (c->dk + c->rope), "the query stride is shorter than a token's heads");

@@ -677,10 +677,10 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
 }  // namespace
 
 extern "C" size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv) {
-    if (!B || !nh || !block_widths(dk, dv)) return 256;
+    if (!B || !nh || !block_widths(dk, dv)) return 0;
     const int per = segment_blocks(T, B, nh, true);
     const size_t n = per ? slots(T, B, per) * nh : 0;
-    return n ? n * dk * dv * 4 + mk_align_up(n * 4, 256) : 256;
+    return n ? n * dk * dv * 4 + mk_align_up(n * 4, 256) : 0;
 }
 
 extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
@@ -689,7 +689,7 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     int st = check_linear(dtype, q, q_stride, k, k_stride, v, v_stride, g, g_stride, T, B, nh, nkh, dk, dv, state, state_out, out);
     if (st != MK_OK) return st;
     MK_REQUIRE(cu || T % B == 0, "without cu every sequence has the same number of tokens");
-    MK_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, "the workspace must be 256-byte aligned");
+    MK_REQUIRE((workspace || mk_linear_attn_workspace_bytes(T, B, nh, dk, dv) == 0) && ((uintptr_t)workspace & 255) == 0, "the workspace must be 256-byte aligned");
     const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out};
     hipStream_t hs = (hipStream_t)stream;
     if (!block_widths(dk, dv)) return dtype == MK_F32 ? launch_token<float>(a, hs) : launch_token<__bf16>(a, hs);

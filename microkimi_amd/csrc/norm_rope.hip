@@ -13,31 +13,16 @@
 
 namespace {
 
-template <typename T> struct Vec8;
-template <> struct Vec8<float> {
-    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
-        const mk_f4 a = *(const mk_f4 *)p, b = *(const mk_f4 *)(p + 4);
+__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
+    *(mk_f4 *)p = mk_f4{v[0], v[1], v[2], v[3]};
+    *(mk_f4 *)(p + 4) = mk_f4{v[4], v[5], v[6], v[7]};
+}
+__device__ __forceinline__ void store8(__bf16 *p, const float (&v)[8]) {
+    mk_b8 a;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
-    }
-    static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
-        *(mk_f4 *)p = mk_f4{v[0], v[1], v[2], v[3]};
-        *(mk_f4 *)(p + 4) = mk_f4{v[4], v[5], v[6], v[7]};
-    }
-};
-template <> struct Vec8<__bf16> {
-    static __device__ __forceinline__ void load(const __bf16 *p, float (&v)[8]) {
-        const mk_b8 a = *(const mk_b8 *)p;
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
-    }
-    static __device__ __forceinline__ void store(__bf16 *p, const float (&v)[8]) {
-        mk_b8 a;
-#pragma unroll
-        for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
-        *(mk_b8 *)p = a;
-    }
-};
+    for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
+    *(mk_b8 *)p = a;
+}
 
 struct NormRopeArgs {
     const void *q, *k;
@@ -69,7 +54,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
             const int h = h0 + grp;
             float x[8];
             if (live && h < h1) {
-                Vec8<T>::load(src + (size_t)h * a.hd + e0, x);
+                mk_load8(src + (size_t)h * a.hd + e0, x);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = 0.0f;
@@ -83,8 +68,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
                         const size_t row = (size_t)p * (a.rot / 2);
                         if (HALVES) {
                             const int i0 = upper ? ri - a.rot / 2 : ri;
-                            Vec8<float>::load(a.cos + row + i0, c);
-                            Vec8<float>::load(a.sin + row + i0, s);
+                            mk_load8(a.cos + row + i0, c);
+                            mk_load8(a.sin + row + i0, s);
                         } else {
                             const mk_f4 cv = *(const mk_f4 *)(a.cos + row + ri / 2), sv = *(const mk_f4 *)(a.sin + row + ri / 2);
 #pragma unroll
@@ -104,7 +89,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
             float w[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) w[i] = 1.0f;
-            if (live && wp) Vec8<float>::load(wp + e0, w);
+            if (live && wp) mk_load8(wp + e0, w);
             float f = 1.0f;
             if (a.norm) {
                 float ss = 0.0f;
@@ -133,7 +118,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) o[i] = y[i];
             }
-            if (live && h < h1) Vec8<T>::store(dst + (size_t)h * a.hd + e0, o);
+            if (live && h < h1) store8(dst + (size_t)h * a.hd + e0, o);
         }
     };
     if (!a.apart || share < a.parts) side((const T *)a.q + (size_t)t * a.qs, (T *)a.qo + (size_t)t * a.qos, a.wq, a.nh);
@@ -189,6 +174,5 @@ extern "C" int mk_dev_qk_norm_rope(int dtype, const void *q, size_t q_stride, si
     a.qs = q_stride, a.ks = k_stride, a.qos = q_out_stride, a.kos = k_out_stride;
     a.wq = wq, a.wk = wk, a.cos = cos, a.sin = sin, a.pos = pos;
     a.n_pos = (int)n_pos, a.nh = (int)nh, a.nkv = (int)nkv, a.hd = (int)hd, a.rot = (int)rot, a.rot_at = (int)rot_at, a.norm = norm ? 1 : 0, a.eps = eps;
-    a.parts = 1;
     return dtype == MK_F32 ? launch_width<float>(a, T, halves, (hipStream_t)stream) : launch_width<__bf16>(a, T, halves, (hipStream_t)stream);
 }

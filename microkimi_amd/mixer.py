@@ -15,6 +15,7 @@ from . import _lib
 from ._lib import BF16, F32, Kv4Cache, check, lib
 
 _TYPES = {torch.float32: F32, torch.bfloat16: BF16}
+_F32 = torch.float32
 _bound = False
 
 
@@ -46,13 +47,13 @@ def _rows(t, name, width=None):
     T, h, w = t.shape
     if t.is_contiguous() and not t.data_ptr() & 15:
         return t, h * w
-    s = t.stride()
-    if (s[2] != 1 and w > 1) or (s[1] != w and h > 1) or s[0] % 8 or (T > 1 and s[0] < h * w) or t.data_ptr() & 15:
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and w > 1) or (s1 != w and h > 1) or (T > 1 and (s0 % 8 or s0 < h * w)) or t.data_ptr() & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()
         return t, h * w
-    return t, s[0] if T > 1 else h * w
+    return t, s0 if T > 1 else h * w
 
 
 def _same(ref, t, name, dtype=None):
@@ -63,22 +64,34 @@ def _same(ref, t, name, dtype=None):
 
 
 def _f32(ref, t, name, shape=None):
-    _same(ref, t, name, torch.float32)
+    if t.dtype is not _F32 or t.get_device() != ref.get_device():
+        _same(ref, t, name, _F32)
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
-    if not t.is_contiguous():
-        t = t.contiguous()
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t
+    t = t.contiguous()
     return t if not t.data_ptr() & 15 else t.clone()
 
 
 def _result(out, ref, shape, name, dtype=None):
     """The caller's output tensor after its checks, or a new one."""
     if out is None:
-        return ref.new_empty(shape) if dtype is None else ref.new_empty(shape, dtype=dtype)
+        if dtype is None:
+            return torch.empty_like(ref, memory_format=torch.contiguous_format) if shape == ref.shape else ref.new_empty(shape)
+        return ref.new_empty(shape, dtype=dtype)
     _same(ref, out, name, dtype)
     if out.shape != shape or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"{name} must be a contiguous, 16-byte aligned {tuple(shape)} tensor")
     return out
+
+
+def _workspace(ref, n):
+    """(n bytes of device memory for a call, their address), or none."""
+    if n == 0:
+        return None, None
+    ws = torch.empty(n, dtype=torch.uint8, device=ref.device)
+    return ws, ws.data_ptr()
 
 
 def _cu_ptr(ref, cu, B, T):
@@ -113,35 +126,39 @@ def qk_norm_rope(q, k, cos=None, sin=None, pos=None, wq=None, wk=None, eps=1e-6,
     if ref is None:
         raise ValueError("q or k must be given")
     dt, hd, T = _code(ref), ref.shape[-1], ref.shape[0]
-    rot = 0
+    rot = n_pos = 0
     if cos is not None:
         if sin is None or pos is None:
             raise ValueError("a rotation needs cos, sin and pos")
         if cos.dim() != 2 or sin.shape != cos.shape:
             raise ValueError("cos and sin must be [n_pos, rot / 2]")
-        rot = 2 * cos.shape[1]
+        n_pos, rot = cos.shape
+        rot *= 2
         cos, sin = _f32(ref, cos, "cos"), _f32(ref, sin, "sin")
     if pos is not None:
         _same(ref, pos, "pos", torch.int32)
         if pos.dim() != 1 or pos.shape[0] != T or not pos.is_contiguous():
             raise ValueError(f"pos must be {T} contiguous values")
-
-    def side(x, w, o, name):
-        if x is None:
-            return None, 0, 0, None, None
-        if x is not ref:
-            _same(ref, x, name)
-            if x.shape[0] != T:
-                raise ValueError("q and k must have the same tokens")
-        xr, stride = _rows(x, name, hd)
-        return xr, stride, x.shape[1], None if w is None else _f32(ref, w, "w" + name, (hd,)), _result(o, x, x.shape, name + "_out")
-
-    (qr, qs, nh, wq, qo), (kr, ks, nkv, wk, ko) = side(q, wq, q_out, "q"), side(k, wk, k_out, "k")
-    st = _start(ref)
-    check(lib.mk_dev_qk_norm_rope(dt, _ptr(qr), qs, nh, _ptr(kr), ks, nkv, T, hd, 1 if norm else 0, _ptr(wq), _ptr(wk), eps, _ptr(cos), _ptr(sin),
-                                  cos.shape[0] if rot else 0, _ptr(pos), rot, hd - rot if rot_at is None else rot_at, 1 if halves else 0, _ptr(qo), nh * hd,
-                                  _ptr(ko), nkv * hd, st))
+    qr, qp, qs, nh, wq, wqp, qo, qop = _heads(ref, q, wq, q_out, T, hd, "q")
+    kr, kp, ks, nkv, wk, wkp, ko, kop = _heads(ref, k, wk, k_out, T, hd, "k")
+    check(lib.mk_dev_qk_norm_rope(dt, qp, qs, nh, kp, ks, nkv, T, hd, 1 if norm else 0, wqp, wkp, eps, _ptr(cos), _ptr(sin), n_pos, _ptr(pos), rot,
+                                  hd - rot if rot_at is None else rot_at, 1 if halves else 0, qop, nh * hd, kop, nkv * hd, _start(ref)))
     return qo, ko
+
+
+def _heads(ref, x, w, out, T, hd, name):
+    """(rows, their address, token stride, heads, weights, their address, output rows, their address) of one side of qk_norm_rope."""
+    if x is None:
+        return None, None, 0, 0, None, None, None, None
+    if x is not ref:
+        _same(ref, x, name)
+        if x.shape[0] != T:
+            raise ValueError("q and k must have the same tokens")
+    xr, stride = _rows(x, name, hd)
+    if w is not None:
+        w = _f32(ref, w, "w" + name, (hd,))
+    out = _result(out, x, x.shape, name + "_out")
+    return xr, xr.data_ptr(), stride, x.shape[1], w, None if w is None else w.data_ptr(), out, out.data_ptr()
 
 
 class KvCache4:
@@ -187,6 +204,7 @@ class KvCache4:
         self.table = Kv4Cache(B, nkv, dk, rope, dv, cap, kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), kr.data_ptr() if rope else None,
                               lens.data_ptr())
         self._ref = C.byref(self.table)
+        self._f32 = lens.new_empty(0, dtype=torch.float32)   # (what new f32 tensors are made like)
 
     def positions(self):
         """Positions held by each sequence (waits for the device)."""
@@ -221,8 +239,8 @@ class KvCache4:
         n = self.cap if n is None else n
         if not 0 <= n <= self.cap:
             raise ValueError("more positions than the cache holds")
-        k = torch.empty((self.B, n, self.nkv, self.dk + self.rope), dtype=torch.float32, device=self.lens.device)
-        v = torch.empty((self.B, n, self.nkv, self.dv), dtype=torch.float32, device=self.lens.device)
+        k = self._f32.new_empty((self.B, n, self.nkv, self.dk + self.rope))
+        v = self._f32.new_empty((self.B, n, self.nkv, self.dv))
         check(lib.mk_dev_kv4_to_f32(self._ref, n, k.data_ptr(), v.data_ptr(), _start(k)))
         return k, v
 
@@ -239,8 +257,8 @@ class KvCache4:
             raise ValueError(f"the query heads must be a multiple of {self.nkv}")
         cup = _cu_ptr(q, cu, self.B, T)
         out = _result(out, q, (T, nh, self.dv), "out")
-        ws = torch.empty(lib.mk_kv4_attn_workspace_bytes(self._ref, T, nh), dtype=torch.uint8, device=q.device)
-        check(lib.mk_dev_kv4_attn(self._ref, dt, q.data_ptr(), stride, T, cup, nh, scale, max_len or 0, ws.data_ptr(), out.data_ptr(), _start(q)))
+        ws, wp = _workspace(q, lib.mk_kv4_attn_workspace_bytes(self._ref, T, nh))
+        check(lib.mk_dev_kv4_attn(self._ref, dt, q.data_ptr(), stride, T, cup, nh, scale, max_len or 0, wp, out.data_ptr(), _start(q)))
         return out
 
 
@@ -287,9 +305,9 @@ def linear_attn(q, k, v, g, state=None, scale=1.0, cu=None, B=None, out=None, st
         raise ValueError("there must be a sequence")
     dt, q, qs, k, ks, v, vs, g, gs, T, nh, nkh, dk, dv, state, state_out, out = _linear_args(q, k, v, g, state, B, out, state_out)
     cup = _cu_ptr(q, cu, B, T)
-    ws = torch.empty(lib.mk_linear_attn_workspace_bytes(T, B, nh, dk, dv), dtype=torch.uint8, device=q.device)
+    ws, wp = _workspace(q, lib.mk_linear_attn_workspace_bytes(T, B, nh, dk, dv))
     check(lib.mk_dev_linear_attn(dt, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), gs, T, cup, B, nh, nkh, dk, dv, scale,
-                                 None if state is None else state.data_ptr(), state_out.data_ptr(), ws.data_ptr(), out.data_ptr(), _start(q)))
+                                 None if state is None else state.data_ptr(), state_out.data_ptr(), wp, out.data_ptr(), _start(q)))
     return out, state_out
 
 

@@ -64,9 +64,12 @@ def test_append_snapshot_and_attention_refusals():
     refused(lib.mk_dev_kv4_attn(c, 0, P, 384, 3, None, 2, 1.0, 0, P, P, None), "same number")
     refused(lib.mk_dev_kv4_attn(c, 0, P, 384, 2, None, 4, 1.0, 0, P, P, None), "shorter")
     refused(lib.mk_dev_kv4_attn(c, 0, P, 384, 2, None, 2, 1.0, 0, P + 16, P, None), "workspace")
-    refused(lib.mk_dev_kv4_attn(c, 0, P, 384, 2, None, 2, 1.0, 0, None, P, None), "null")
+    refused(lib.mk_dev_kv4_attn(c, 0, P, 384, 2, None, 2, 1.0, 0, P, None, None), "null")
+    long = cache(cap=4096)
+    assert lib.mk_kv4_attn_workspace_bytes(long, 2, 2) > 0
+    refused(lib.mk_dev_kv4_attn(long, 0, P, 384, 2, None, 2, 1.0, 0, None, P, None), "null")
     assert lib.mk_dev_kv4_attn(c, 0, None, 384, 0, None, 2, 1.0, 0, None, None, None) == 0   # no rows: nothing to do
-    assert lib.mk_kv4_attn_workspace_bytes(c, 1, 96) >= 256
+    assert lib.mk_kv4_attn_workspace_bytes(c, 1, 96) == 0      # one piece: nothing to keep
 
 
 def linear(dtype=0, q=P, qs=256, k=P, ks=256, v=P, vs=256, g=P, gs=2, T=4, cu=None, B=2, nh=2, nkh=2, dk=128, dv=128, state=P, state_out=P, ws=P, out=P):
@@ -76,7 +79,7 @@ def linear(dtype=0, q=P, qs=256, k=P, ks=256, v=P, vs=256, g=P, gs=2, T=4, cu=No
 @pytest.mark.parametrize("bad,word", [(dict(dtype=9), "dtype"), (dict(B=0), "count"), (dict(T=5), "same number"), (dict(nkh=0), "key heads"), (dict(nh=3), "key heads"),
                                       (dict(dk=4), "multiples of 8"), (dict(dv=264), "256"), (dict(v=None), "null"), (dict(state_out=None), "null"),
                                       (dict(g=None), "null"), (dict(qs=250), "multiples of 8"), (dict(vs=248), "shorter"), (dict(gs=1), "shorter"),
-                                      (dict(k=P + 8), "aligned"), (dict(state=P + 4), "aligned"), (dict(ws=None), "workspace"), (dict(ws=P + 16), "workspace")])
+                                      (dict(k=P + 8), "aligned"), (dict(state=P + 4), "aligned"), (dict(ws=None, T=2048), "workspace"), (dict(ws=P + 16), "workspace")])
 def test_linear_refusals(bad, word):
     refused(linear(**bad), word)
     if not {"T", "ws"} & set(bad):
