@@ -557,3 +557,68 @@ def test_a_call_without_sequences_is_refused():
             mixer.linear_attn(x, x, x, g, **kw)
     with pytest.raises(ValueError):
         mixer.KvCache4(0, 1, 32, 32, 4)
+
+
+# ------------------------------------------------------------------------------------------- offsets that pass 32 bits
+
+def test_norm_rope_beyond_four_gigabytes():
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    T, nh = 2 ** 18 + 3, 64
+    q = torch.empty((T, nh, 128), dtype=torch.bfloat16, device="cuda").normal_()     # 2^31 values and some
+    k = torch.empty((T, 1, 128), dtype=torch.bfloat16, device="cuda").normal_()
+    cos, sin = mixer.rope_table(4096, 64)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") % 4096
+    qo, ko = mixer.qk_norm_rope(q, k, cos, sin, pos, halves=True)
+    for a, b in ((0, 3), (T // 2, T // 2 + 2), (T - 3, T)):
+        wq, wk = mixer.qk_norm_rope(q[a:b], k[a:b], cos, sin, pos[a:b], halves=True)
+        assert torch.equal(qo[a:b], wq) and torch.equal(ko[a:b], wk)
+    del q, k, qo, ko
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_kv4_cache_beyond_four_gigabytes(new):
+    """A cache at its largest capacity, zeros but for the last rows, whose scores stand far above: the last head's K and V lie
+    behind the 4 GiB of the others."""
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    rng = np.random.default_rng(5)
+    nkv, cap = 9, 8388607
+    c = mixer.KvCache4(1, nkv, 128, 128, cap, rope=64)
+    assert c.kq.numel() > 2 ** 32
+    c.lens.fill_(cap - new)
+    k, v = rows(rng, (new, nkv, 192), "f32"), rows(rng, (new, nkv, 128), "f32")
+    c.push(to_dev(k), to_dev(v))
+    kk, vv = held(k, 128, v)
+    q = np.repeat(kk[:1].astype(np.float32), new, 0)          # the first new row's own K: |k|^2 against a few |k| elsewhere
+    scale = 40.0 / float((kk[0] ** 2).sum(-1).min())
+    out = host(c.attn(to_dev(q), scale))
+    for i in range(new):
+        s = np.einsum("hw,jhw->jh", q[i].astype(np.float64), kk[:i + 1]) * scale
+        p = np.exp(s)
+        den = p.sum(0) + (cap - new)
+        want, mag = np.einsum("jh,jhd->hd", p, vv[:i + 1]) / den[:, None], np.einsum("jh,jhd->hd", p, np.abs(vv[:i + 1])) / den[:, None]
+        # as in mixer_ref.attn for the rows that count; the zeros' share of the sum is below 8.4e6 e^-40 = 4e-11
+        ds = 194 * (np.abs(q[i].astype(np.float64)) * np.abs(kk[:i + 1])).sum(-1).max() * scale
+        within(out[i], want, (2 * ds + new + 16) * mag * U32 + 1e-30, f"row {i}")
+    del c
+    torch.cuda.empty_cache()
+
+
+def test_linear_beyond_four_gigabytes():
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    T, nh = 2 ** 19 + 100, 32
+    q = torch.empty((T, 1, 64), dtype=torch.bfloat16, device="cuda").normal_()
+    k = torch.empty((T, 1, 64), dtype=torch.bfloat16, device="cuda").normal_()
+    v = torch.empty((T, nh, 128), dtype=torch.bfloat16, device="cuda").normal_()      # 2^31 values and some
+    g = torch.full((nh,), -0.5, device="cuda")
+    out, S = mixer.linear_attn(q, k, v, g)
+    for end in (T, T // 2):                                     # e^-220 of what lies 440 tokens back: nothing
+        want, W = mixer.linear_attn(q[end - 704:end], k[end - 704:end], v[end - 704:end], g)
+        assert rel_l2(host(out[end - 256:end]), host(want[-256:])) <= 4 * U16
+    want, W = mixer.linear_attn(q[-704:], k[-704:], v[-704:], g)
+    assert rel_l2(host(S), host(W)) <= 1e-5
+    del q, k, v, out
+    torch.cuda.empty_cache()

@@ -130,3 +130,18 @@ def test_tables_hold_far_positions():
         for i in (0, 1, 31):
             a = p * 10000.0 ** (-2 * i / 64)
             assert abs(float(cos[p, i]) - math.cos(a)) <= 2 ** -24 + 1e-9 and abs(float(sin[p, i]) - math.sin(a)) <= 2 ** -24 + 1e-9
+
+
+def test_the_cache_struct_is_the_same_in_the_header_the_binding_and_the_shim():
+    import pathlib
+    import re
+    root = pathlib.Path(__file__).resolve().parents[1]
+    body = re.search(r"typedef struct \{([^}]*)\} mk_kv4_cache;", (root / "include/mk_hip.h").read_text()).group(1)
+    header = []
+    for kind, names in re.findall(r"(\w+) ([^;]+);", body):
+        header += [(n.strip(" *"), "*" in n, kind) for n in names.split(",")]
+    body = re.search(r"struct MkKv4Cache \{([^}]*)\}", (root / "rust/hip.rs").read_text()).group(1)
+    rust = [(n, t.startswith("*mut"), t.split()[-1]) for n, t in re.findall(r"(\w+): ([^,\n]+)", body)]
+    kinds = {"size_t": "usize", "uint8_t": "u8", "uint16_t": "u16", "int32_t": "i32"}
+    assert rust == [(n, p, kinds[k]) for n, p, k in header]
+    assert [(n, t is C.c_size_t) for n, t in Kv4Cache._fields_] == [(n, not p) for n, p, _ in header]
