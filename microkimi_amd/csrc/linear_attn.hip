@@ -20,6 +20,7 @@ struct LinArgs {
     const float *state;     // may be null: zeros
     float *state_out;
     void *out;              // [T][nh][dv]
+    int slices;             // workgroups that share out a head's columns of dv
     __device__ __forceinline__ int at(int b) const { return cu ? min(max(cu[b], 0), T) : (int)((int64_t)T / B * b); }
 };
 
@@ -335,7 +336,8 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
     __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
     __shared__ int bad_l;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int h = blockIdx.x % a.nh, slot = blockIdx.x / a.nh, hk = h / (a.nh / a.nkh);
+    const int slices = MODE == BOTH ? a.slices : 1, dv = MODE == BOTH ? a.dv : DV;
+    const int hs = blockIdx.x % (a.nh * slices), h = hs / slices, col0 = (hs - h * slices) * DV, slot = blockIdx.x / (a.nh * slices), hk = h / (a.nh / a.nkh);
     int b = slot, c0 = 0;
     if (MODE != BOTH) {  // the last sequence whose slots begin at this one or before
         int lo = 0, hi = a.B;
@@ -349,7 +351,7 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
     }
     const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0), nch = (len + CH - 1) / CH, c1 = MODE == BOTH ? nch : min(c0 + sg.per, nch);
     if (MODE != BOTH && c0 >= c1) return;
-    const size_t sh = (size_t)slot * a.nh + h, sbase = ((size_t)b * a.nh + h) * DK * DV + 16 * NT * wave + n;
+    const size_t sh = (size_t)slot * a.nh + h, sbase = ((size_t)b * a.nh + h) * DK * dv + col0 + 16 * NT * wave + n;
     mk_f4 S[KT][NT];
     mk_f4 *mine = sg.local + sh * KT * (DV * 4) + 64 * NT * wave + lane;
 #pragma unroll
@@ -361,10 +363,10 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
                 S[kt][t] = mine[kt * (DV * 4) + 64 * t];
             } else if (MODE == BOTH && a.state) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) S[kt][t][j] = a.state[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * DV];
+                for (int j = 0; j < 4; j++) S[kt][t][j] = a.state[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * dv];
             }
         }
-    const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * DV;
+    const T *qp = (const T *)a.q + (size_t)hk * DK, *kp = (const T *)a.k + (size_t)hk * DK, *vp = (const T *)a.v + (size_t)h * dv + col0;
     mk_v4u kr[KP], vr[VP], qr[OUT ? KP : 1];
     float gr;
     // A block's rows into registers: a scalar base, a lane offset that never changes, and a scalar step from piece to piece.  Rows behind the
@@ -515,7 +517,7 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
             for (int j = 0; j < 4; j++) {
                 const int tok = c * CH + 16 * j + n;
                 if (tok < len) {
-                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * DV + 16 * NT * wave + 4 * g;
+                    T *dst = (T *)a.out + ((size_t)(t0 + tok) * a.nh + h) * dv + col0 + 16 * NT * wave + 4 * g;
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         const mk_f4 x = o[t][j];
@@ -581,7 +583,7 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
         for (int t = 0; t < NT; t++) {
             if constexpr (MODE == BOTH) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) a.state_out[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * DV] = S[kt][t][j];
+                for (int j = 0; j < 4; j++) a.state_out[sbase + 16 * t + (size_t)(16 * kt + 4 * g + j) * dv] = S[kt][t][j];
             } else {
                 mine[kt * (DV * 4) + 64 * t] = S[kt][t];
             }
@@ -630,18 +632,21 @@ __global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg 
 // Equal lengths (no cu) are better off without from 192 heads on (bfloat16, 128 x 128; without / with): 192 heads of 400 tokens 43 / 64 us, of 1500
 // tokens 135 / 162 us; 128 heads of 400 tokens 41 / 48 us, of 1500 tokens 125 / 90 us.  What cu holds is not known here: up to 256 heads it
 // is taken for ragged (8 sequences of 24 heads, 1 .. 6000 tokens long: 340 / 125 us).
-int segment_blocks(size_t T, size_t B, size_t nh, bool ragged) {
+// A sequence needs four blocks on average, six of 128 bfloat16 columns, which two workgroups share when they are few (32 heads of 128 x 128
+// without / with: 256 tokens 20 / 24 us, 400 tokens 32 / 29 us; in f32 256 tokens 42 / 45 us, 320 tokens 53 / 47 us).
+int segment_blocks(size_t T, size_t B, size_t nh, size_t dv, bool bf16, bool ragged) {
     const size_t blocks = (T + CH - 1) / CH;
-    if (B * nh > (ragged ? 256 : 191) || blocks < 4 * B) return 0;
+    if (B * nh > (ragged ? 256 : 191) || blocks < (bf16 && dv == 128 ? 6 : 4) * B) return 0;
     const size_t per = (blocks * nh + 511) / 512;
     return (int)(per < 2 ? 2 : per);
 }
 size_t slots(size_t T, size_t B, int per) { return T / ((size_t)CH * per) + B; }
+constexpr size_t SLICED = 128;
 bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv == 64 || dv == 128); }
 
 template <typename T, int DK, int DV>
 int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
-    const dim3 grid((unsigned)(a.nh * (sg.per ? slots(a.T, a.B, sg.per) : (size_t)a.B)));
+    const dim3 grid((unsigned)(a.nh * (sg.per ? slots(a.T, a.B, sg.per) : (size_t)a.B * a.slices)));
     int e;
     if (sg.per == 0) {
         hipLaunchKernelGGL((linear_block_kernel<T, DK, DV, BOTH>), grid, dim3(DV * 4 / tiles<T, DK, DV, BOTH>()), 0, st, a, sg);
@@ -655,7 +660,13 @@ int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
     return mk_launch_status("linear_block");
 }
 template <typename T>
-int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
+int launch_blocks(LinArgs a, const LinSeg &sg, hipStream_t st) {
+    // While heads leave compute units free, two workgroups share a head of 128 columns (32 heads of 128 x 128, 70 tokens: f32 30 -> 23 us, bfloat16
+    // 13.3 -> 11.6 us; 128 heads of 100 tokens 15.4 -> 14.0 us; 192 f32 heads would take 33 for 20 us)
+    if (sg.per == 0 && a.dv == 128 && (size_t)a.B * a.nh <= SLICED) {
+        a.slices = 2;
+        return a.dk == 64 ? launch_blocks<T, 64, 64>(a, sg, st) : launch_blocks<T, 128, 64>(a, sg, st);
+    }
     if (a.dk == 64) return a.dv == 64 ? launch_blocks<T, 64, 64>(a, sg, st) : launch_blocks<T, 64, 128>(a, sg, st);
     return a.dv == 64 ? launch_blocks<T, 128, 64>(a, sg, st) : launch_blocks<T, 128, 128>(a, sg, st);
 }
@@ -678,7 +689,7 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
 
 extern "C" size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv) {
     if (!B || !nh || !block_widths(dk, dv)) return 0;
-    const int per = segment_blocks(T, B, nh, true);
+    const int per = segment_blocks(T, B, nh, dv, false, true);
     const size_t n = per ? slots(T, B, per) * nh : 0;
     return n ? n * dk * dv * 4 + mk_align_up(n * 4, 256) : 0;
 }
@@ -690,10 +701,10 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     if (st != MK_OK) return st;
     MK_REQUIRE(cu || T % B == 0, "without cu every sequence has the same number of tokens");
     MK_REQUIRE((workspace || mk_linear_attn_workspace_bytes(T, B, nh, dk, dv) == 0) && ((uintptr_t)workspace & 255) == 0, "the workspace must be 256-byte aligned");
-    const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out};
+    const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out, 1};
     hipStream_t hs = (hipStream_t)stream;
     if (!block_widths(dk, dv)) return dtype == MK_F32 ? launch_token<float>(a, hs) : launch_token<__bf16>(a, hs);
-    LinSeg sg{segment_blocks(T, B, nh, cu != nullptr), (mk_f4 *)workspace, nullptr};
+    LinSeg sg{segment_blocks(T, B, nh, dv, dtype == MK_BF16, cu != nullptr), (mk_f4 *)workspace, nullptr};
     const size_t n = (sg.per ? slots(T, B, sg.per) : B) * nh;
     sg.decay = sg.per ? (float *)((uint8_t *)workspace + n * dk * dv * 4) : nullptr;
     MK_REQUIRE(n <= MAX_GROUPS / 2, "too many heads and sequences in one call");
@@ -705,6 +716,6 @@ extern "C" int mk_dev_linear_attn_step(int dtype, const void *q, size_t q_stride
                                        const float *state, float *state_out, void *out, void *stream) {
     int st = check_linear(dtype, q, q_stride, k, k_stride, v, v_stride, g, g_stride, B, B, nh, nkh, dk, dv, state, state_out, out);
     if (st != MK_OK) return st;
-    const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, nullptr, (int)B, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out};
+    const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, nullptr, (int)B, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out, 1};
     return dtype == MK_F32 ? launch_step<float, 16>(a, (hipStream_t)stream) : launch_step<__bf16, 16>(a, (hipStream_t)stream);
 }
