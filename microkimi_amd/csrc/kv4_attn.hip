@@ -846,6 +846,9 @@ void plan_many(AttnArgs &a, size_t pairs, size_t len, size_t rows, size_t elem, 
     }
 }
 
+// results of n chunks
+size_t piece_bytes(size_t n, size_t rows, size_t dv) { return mk_align_up(n * rows * dv * 4, 256) + 2 * mk_align_up(n * rows * 4, 256); }
+
 size_t column_tiles(const mk_kv4_cache *c, size_t T, const int32_t *cu, size_t group, size_t ct) {
     return cu ? T * group / ct + c->B : c->B * ((T / c->B * group + ct - 1) / ct);
 }
@@ -876,7 +879,7 @@ extern "C" size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, s
     const Form form = form_of(c, T, group);
     const size_t pairs = c->nkv * (cols / form ? cols / form : 1);
     const size_t n = form == MANY ? most_many(pairs, c->cap) : uncut(form, T, c->B, pairs) ? 1 : most_few(pairs, c->cap);
-    return n <= 1 ? 0 : mk_align_up(n * T * nh * c->dv * 4, 256) + 2 * mk_align_up(n * T * nh * 4, 256);
+    return n <= 1 ? 0 : piece_bytes(n, T * nh, c->dv);
 }
 
 extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_stride, size_t T, const int32_t *cu, size_t nh, float scale,
@@ -900,6 +903,7 @@ extern "C" int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, 
     else if (uncut(form, T, c->B, pairs)) a.chunk = (int)len, a.n_splits = 1;
     else plan_few(a, pairs, len);
     MK_REQUIRE(a.n_splits == 1 || (T * nh + 3) / 4 <= MAX_GROUPS, "too many query rows in one call");
+    MK_REQUIRE(a.n_splits == 1 || piece_bytes(a.n_splits, T * nh, c->dv) <= mk_kv4_attn_workspace_bytes(c, T, nh), "chunks beyond the workspace");
     uint8_t *w = (uint8_t *)workspace;
     a.po = (float *)w;
     w += mk_align_up((size_t)a.n_splits * T * nh * c->dv * 4, 256);

@@ -626,6 +626,13 @@ __global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg 
     for (int j = 0; j < 4; j++) a.state_out[at + (size_t)j * DV] = S[j];
 }
 
+size_t least_segment(size_t T, size_t nh) {  // no call takes shorter ones: the workspace is measured by this
+    const size_t per = ((T + CH - 1) / CH * nh + 511) / 512;
+    return per < 2 ? 2 : per;
+}
+size_t slots(size_t T, size_t B, size_t per) { return T / (CH * per) + B; }
+size_t segment_bytes(size_t n, size_t dk, size_t dv) { return n * dk * dv * 4 + mk_align_up(n * 4, 256); }  // of n (slot, head) pairs
+
 // Blocks of a segment, 0: no segments.  Without them a (sequence, head) is one workgroup; with them the keys and values are read twice
 // (local states first, then the outputs from the right states), and a long sequence beside short ones spreads over the device.
 // As many as two workgroups a compute unit ask for: 8192 tokens of 32 heads 118 us, as 768 or 1024 workgroups 132 and 136 us.
@@ -634,13 +641,18 @@ __global__ __launch_bounds__(DV * 4) void linear_carry_kernel(LinArgs a, LinSeg 
 // is taken for ragged (8 sequences of 24 heads, 1 .. 6000 tokens long: 340 / 125 us).
 // A sequence needs four blocks on average, six of 128 bfloat16 columns, which two workgroups share when they are few (32 heads of 128 x 128
 // without / with: 256 tokens 20 / 24 us, 400 tokens 32 / 29 us; in f32 256 tokens 42 / 45 us, 320 tokens 53 / 47 us).
-int segment_blocks(size_t T, size_t B, size_t nh, size_t dv, bool bf16, bool ragged) {
+// f32 heads wider than 64 x 64 leave room for one workgroup a compute unit: longer segments of equal sequences, so that all of them run at
+// once (2048 tokens of 32 heads of 128 x 128: 91 us, in segments of two blocks 100; 3241 of 24 heads 123 and 132 us).
+int segment_blocks(size_t T, size_t B, size_t nh, size_t dk, size_t dv, bool bf16, bool ragged) {
     const size_t blocks = (T + CH - 1) / CH;
     if (B * nh > (ragged ? 256 : 191) || blocks < (bf16 && dv == 128 ? 6 : 4) * B) return 0;
-    const size_t per = (blocks * nh + 511) / 512;
-    return (int)(per < 2 ? 2 : per);
+    size_t per = least_segment(T, nh);
+    if (!ragged && !bf16 && dk + dv > 128) {
+        const size_t most = 256 / (B * nh), even = ((T / B + CH - 1) / CH + most - 1) / most;
+        per = even > per ? even : per;
+    }
+    return (int)per;
 }
-size_t slots(size_t T, size_t B, int per) { return T / ((size_t)CH * per) + B; }
 constexpr size_t SLICED = 128;
 bool block_widths(size_t dk, size_t dv) { return (dk == 64 || dk == 128) && (dv == 64 || dv == 128); }
 
@@ -689,9 +701,8 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
 
 extern "C" size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv) {
     if (!B || !nh || !block_widths(dk, dv)) return 0;
-    const int per = segment_blocks(T, B, nh, dv, false, true);
-    const size_t n = per ? slots(T, B, per) * nh : 0;
-    return n ? n * dk * dv * 4 + mk_align_up(n * 4, 256) : 0;
+    const size_t n = B * nh <= 256 && (T + CH - 1) / CH >= 4 * B ? slots(T, B, least_segment(T, nh)) * nh : 0;
+    return n ? segment_bytes(n, dk, dv) : 0;
 }
 
 extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v, size_t v_stride, const float *g,
@@ -704,10 +715,11 @@ extern "C" int mk_dev_linear_attn(int dtype, const void *q, size_t q_stride, con
     const LinArgs a{q, k, v, q_stride, k_stride, v_stride, g, g_stride, cu, (int)T, (int)B, (int)nh, (int)nkh, (int)dk, (int)dv, scale, state, state_out, out, 1};
     hipStream_t hs = (hipStream_t)stream;
     if (!block_widths(dk, dv)) return dtype == MK_F32 ? launch_token<float>(a, hs) : launch_token<__bf16>(a, hs);
-    LinSeg sg{segment_blocks(T, B, nh, dv, dtype == MK_BF16, cu != nullptr), (mk_f4 *)workspace, nullptr};
+    LinSeg sg{segment_blocks(T, B, nh, dk, dv, dtype == MK_BF16, cu != nullptr), (mk_f4 *)workspace, nullptr};
     const size_t n = (sg.per ? slots(T, B, sg.per) : B) * nh;
     sg.decay = sg.per ? (float *)((uint8_t *)workspace + n * dk * dv * 4) : nullptr;
     MK_REQUIRE(n <= MAX_GROUPS / 2, "too many heads and sequences in one call");
+    MK_REQUIRE(sg.per == 0 || segment_bytes(n, dk, dv) <= mk_linear_attn_workspace_bytes(T, B, nh, dk, dv), "segments beyond the workspace");
     return dtype == MK_F32 ? launch_blocks<float>(a, sg, hs) : launch_blocks<__bf16>(a, sg, hs);
 }
 
