@@ -123,17 +123,17 @@ __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, At
 // position, which is one block (one scale byte) at DK = 128.
 //
 // 4-bit values become bfloat16 exactly (two significant bits, and the exponent of an f32), so the products are exact in f32.
-// f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as P terms (few
-// columns) or PM terms (many): three for f32 results.  For bfloat16 results, whose own rounding is up to 2^-9, two (17 bits) where the
-// product costs no time (few columns are bound by memory: one term 59.7, two 59.8 us at 96 heads x 16384 positions), and one where it
-// does (512 rows behind 3584 positions: one term 160, two 192 us): its roundings, 2^-9 of each weight, are as large as the result's
-// at most and average out over the positions.
+// f32 queries enter as three bfloat16 terms (24 bits: every bit of the value).  A weight p of the softmax enters as P terms: three for
+// f32 results, two for bfloat16 ones (17 bits, so that the result's own rounding, 2^-8 of it at most, is the only one that counts).  One term
+// would cost a second whole rounding: a result with values of both signs shrinks with the sum of its weights' errors, which is why these
+// do not average out (2.3e-3 against 1.7e-3 over 4096 positions).  With few columns the second term costs no time (bound by memory: one term 59.7, two 59.8
+// us at 96 heads x 16384 positions), with many it does (512 rows behind 3584 positions: one term 165, two 200 us).
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float FAR = 1048576.0f;  // 2^20: weights up to this above the reference point are summed as they are
 
 template <typename T> struct Terms;
-template <> struct Terms<float> { static constexpr int Q = 3, P = 3, PM = 3; };
-template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2, PM = 1; };
+template <> struct Terms<float> { static constexpr int Q = 3, P = 3; };
+template <> struct Terms<__bf16> { static constexpr int Q = 1, P = 2; };
 
 __device__ __forceinline__ mk_f4 mfma(mk_b8 a, mk_b8 b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -494,9 +494,9 @@ __global__ __launch_bounds__(256, DK == 256 && sizeof(T) == 4 ? 1 : 2) void kv4_
 
 // ----------------------------------------------------------------------- many query columns: the workgroup shares K and V
 //
-// 512 rows behind 3584 positions, 96 heads of 128 + 64 | 128 in bfloat16 (121 GFLOP): 160 us, 756 TFLOP/s (a large library product:
-// 1085).  Operand reads from LDS (80 KB a step and workgroup) alone take 96 us, vector issue 72, the matrix cores 49; without the fetches
-// it is 141 us.  32 columns a wave would halve the reads, but 128 columns a workgroup leave 384 of them to 512 places.
+// 512 rows behind 3584 positions, 96 heads of 128 + 64 | 128 in bfloat16 (121 GFLOP): 200 us, 605 TFLOP/s (a large library product:
+// 1085).  Operand reads from LDS (80 KB a step and workgroup) alone take 96 us, the matrix cores 69 (49 without the weights' second term).
+// 32 columns a wave would halve the reads, but 128 columns a workgroup leave 384 of them to 512 places.
 //
 // One workgroup: (tile of 64 query columns, 16 a wave; kv head; chunk of the context), 32 positions a step.  Waves 0 and 1 turn the K
 // rows of 16 positions each into bfloat16 operands in LDS, waves 2 and 3 the V rows (as in the kernel above, so no transposed read
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256, DK == 256 && sizeof(T) == 4 ? 1 : 2) void kv4_
 //   scores of step h + 1 on the matrix cores, beside them the weights of step h on the vector units
 //   O += V P of step h, beside it the operands of K of step h + 2 and of V of step h + 1; the bytes of the step after are asked for
 // The statements stand in the order in which they are to be issued (sched_barrier keeps it): a matrix instruction runs for 16 cycles,
-// in which the wave can issue what does not wait for it; operands are read from LDS three products ahead.
+// in which the wave can issue what does not wait for it; operands are read from LDS three (scores) or two (outputs) of them ahead.
 // A wave's share of a step: the K, or the V rows of 16 positions.  Positions past `last` are read as `last`.
 template <int DK, int R> struct KQuarter {
     static constexpr int KL = DK == 256 ? 2 : 1;
@@ -583,12 +583,12 @@ template <typename T, int N> __device__ __forceinline__ void store_run(void *out
 }
 
 // Workgroups of the kernel below that a compute unit holds (registers; at width 256 two instead of one: 512 rows at 4096 positions, 16 heads,
-// 73 us instead of 113).
+// 73 us instead of 113 with one-term weights, 76 us with two).
 constexpr int many_per_cu(size_t elem, size_t dk) { return dk == 256 ? (elem == 4 ? 1 : 2) : elem == 4 ? 2 : 3; }
 
 template <typename T, int DK, int R, int DV>
 __global__ __launch_bounds__(256, many_per_cu(sizeof(T), DK)) void kv4_attn_many_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
-    constexpr int NS = DK / 32, NR = R / 32, NF = NS + NR, NK = 2 * NF, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::PM;
+    constexpr int NS = DK / 32, NR = R / 32, NF = NS + NR, NK = 2 * NF, NT = DV / 16, QT = Terms<T>::Q, PT = Terms<T>::P;
     __shared__ mk_b8 k_l[2][2][NF][64], v_l[2][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % c.nkv, G = a.nh / c.nkv;
@@ -690,29 +690,34 @@ __global__ __launch_bounds__(256, many_per_cu(sizeof(T), DK)) void kv4_attn_many
             }
             l += sum;
 #pragma unroll
-            for (int k = 0; k < 3; k++) ring[k] = v_l[buf][k][lane];
+            for (int k = 0; k < 2; k++) ring[k] = v_l[buf][k][lane];
             mk_b8 pf[PT];
             split8<PT>(p, pf);
             __builtin_amdgcn_sched_barrier(0);
-            auto out_tile = [&](int t) {
-                if (t + 3 < NT) ring[(t + 3) & 3] = v_l[buf][t + 3][lane];
+            // (two sums in turn, as above)
+            auto out_tiles = [&](int t) {
 #pragma unroll
-                for (int k = 0; k < PT; k++) o[t] = mfma(ring[t & 3], pf[k], o[t]);
+                for (int i = 2; i < 4; i++)
+                    if (t + i < NT) ring[(t + i) & 3] = v_l[buf][t + i][lane];
+#pragma unroll
+                for (int k = 0; k < PT; k++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) o[t + i] = mfma(ring[(t + i) & 3], pf[k], o[t + i]);
             };
             if (k_wave) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    out_tile(t);
+                for (int t = 0; t < NT; t += 2) {
+                    out_tiles(t);
 #pragma unroll
-                    for (int e = NF * t / NT; e < NF * (t + 1) / NT; e++) kx.store(k_l[buf][half], e, lane);
+                    for (int e = NF * t / NT; e < NF * (t + 2) / NT; e++) kx.store(k_l[buf][half], e, lane);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 fetch_k(j + 96);
             } else {
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    out_tile(t);
-                    if (t % 2 == 0) vx.store(v_l[buf ^ 1], t / 2, half, lane);
+                for (int t = 0; t < NT; t += 2) {
+                    out_tiles(t);
+                    vx.store(v_l[buf ^ 1], t / 2, half, lane);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 fetch_v(j + 64);
@@ -821,9 +826,9 @@ size_t most_few(size_t pairs, size_t cap) {
 }
 
 // Many columns: the number of chunks with the least estimated time, of those that make no more than about 1024 workgroups.  A step of 32
-// positions takes 0.3 + 0.5 us for every 256 values of K and V (f32: 1.8 times that); a second workgroup on a compute unit costs 5 %, a third
-// 20 % more; a merge takes 8 us and its results' way to memory and back.  (96 heads over 4096 positions: 192 rows 129 us uncut, 103 in two
-// chunks, 300 rows 133 and 165; 200 rows of 48 heads over 16000: 194 us in four chunks, 143 in six.)
+// positions takes 0.38 + 0.62 us for every 256 values of K and V (f32: 1.5 times that); a second workgroup on a compute unit costs 5 %, a third
+// 20 % more; a merge takes 8 us and its results' way to memory and back.  (96 heads over 4096 positions: 192 rows 142 us uncut, 118 in two
+// chunks, 300 rows 145 and 185; 200 rows of 48 heads over 16000: 277 us in two chunks, 206 in four, 227 in six.)
 size_t most_many(size_t pairs, size_t cap) {
     size_t n = (1024 + pairs - 1) / pairs;
     n = n < cap / 256 ? n : cap / 256;
@@ -833,7 +838,7 @@ size_t most_many(size_t pairs, size_t cap) {
 void plan_many(AttnArgs &a, size_t pairs, size_t len, size_t rows, size_t elem, const mk_kv4_cache *c) {
     const size_t at_once = many_per_cu(elem, c->dk);
     const double share[4] = {0.0, 1.0, 1.05, 1.25};  // time of 0 .. 3 workgroups on a compute unit
-    const double step = (0.3 + 0.5 * (c->dk + c->rope + c->dv) / 256) * (elem == 4 ? 1.8 : 1.0);
+    const double step = (0.38 + 0.62 * (c->dk + c->rope + c->dv) / 256) * (elem == 4 ? 1.5 : 1.0);
     double best = 0.0;
     a.chunk = (int)len, a.n_splits = 1;
     for (size_t n = 1; n <= most_many(pairs, len); n++) {

@@ -622,3 +622,31 @@ def test_linear_beyond_four_gigabytes():
     assert rel_l2(host(S), host(W)) <= 1e-5
     del q, k, v, out
     torch.cuda.empty_cache()
+
+
+# --------------------------------------------------------------------------------------- bfloat16 results are rounded once
+
+def rounded_once(got, want, before, what):
+    """got is a value within `before` of want, rounded to bfloat16."""
+    within(got, want, before + U16 * (np.abs(want) + before) + 1e-30, what)
+
+
+@pytest.mark.parametrize("lens,news,nh,nkv,dk,rope", [([700, 90], [90, 33], 4, 2, 128, 64), ([1200], [200], 8, 1, 64, 0), ([300, 40], [1, 1], 40, 2, 128, 0),
+                                                      ([20, 9], [1, 9], 4, 2, 64, 64), ([260], [70], 2, 2, 256, 0), ([900, 7], [1, 1], 6, 2, 128, 0)])
+def test_kv4_a_bfloat16_result_is_rounded_once(lens, news, nh, nkv, dk, rope):
+    """Prompts, wide groups, small caches and plain decoding.  A weight may enter its product as two bfloat16 terms: what is left of it is
+    half a step of half a step, U16^2."""
+    from microkimi_amd import mixer
+    rng = np.random.default_rng(31 + sum(lens))
+    c = mixer.KvCache4(len(lens), nkv, dk, dk, max(lens), rope=rope)
+    k, v = split(rng, lens, (nkv, dk + rope), "bf16"), split(rng, lens, (nkv, dk), "bf16")
+    c.push(to_dev(np.concatenate(k), "bf16"), to_dev(np.concatenate(v), "bf16"), cu=cu_of(lens))
+    q = rows(rng, (sum(news), nh, dk + rope), "bf16")
+    scale = (dk + rope) ** -0.5
+    got, t = host(c.attn(to_dev(q, "bf16"), scale, cu=cu_of(news))), 0
+    for b in range(len(lens)):
+        kk, vv = held(k[b], dk, v[b])
+        for i in range(news[b]):
+            want, bound, mag = ref.attn(q[t], kk, vv, lens[b] - news[b] + i, scale)
+            rounded_once(got[t], want, bound * U32 + U16 ** 2 * mag, f"sequence {b} row {i}")
+            t += 1
