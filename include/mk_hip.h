@@ -418,7 +418,8 @@ int mk_dev_mla_heads_q8_attn(const int8_t *kq, const float *ks, const float *kr,
 /* ------------------------------------------- device level: token mixers */
 
 /* These calls have no counterpart in the reference's hot path; rows are f32 or bfloat16 (dtype: MK_F32, MK_BF16), sums, norms,
- * softmax statistics and states f32, and a bfloat16 result is rounded once.
+ * softmax statistics and states f32, and a bfloat16 result is rounded once (an f32 operand of a product that bfloat16 rows make on the
+ * matrix cores - softmax weights, weighted scores, a state - enters as two bfloat16 terms, 17 bits, or three).
  *
  * A batch of sequences: the rows of a call lie one behind the other, cu [B + 1] int32 (device) says where each sequence's
  * begin and the last one's end; cu NULL: T / B rows each (T % B == 0).  Entries of cu outside 0 .. T are taken as the nearer

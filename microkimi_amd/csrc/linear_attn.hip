@@ -197,13 +197,14 @@ int launch_token(const LinArgs &a, hipStream_t st) {
 //   scores   A = K rows, B = Q rows               -> (key, query), weighted by the decay, masked, to LDS (six operands, shared out)
 //   out      A = S^T, B = Q^T; times e^{b_i}; A = V^T, B = scores     -> (dv, token)
 //   state    A = K^T, B = weighted V^T            -> (dk, dv)
-// bfloat16 rows: S and the weighted scores are rounded to bfloat16 for the products of the output (whose own rounding is as large);
+// bfloat16 rows: S and the weighted scores enter the products of the output as two bfloat16 terms each (17 bits, so that the result is rounded
+// once; as one term, whose rounding is as large as the result's own, the error against 64 bits is 2.3e-3 instead of 1.7e-3);
 // the state itself is f32 through and through, so its weighted values enter in three bfloat16 terms (24 bits).
 // f32 rows: the same on the f32 matrix instruction (in three bfloat16 terms, six products: 128 x 128 heads 100 -> 95 us, but 64 x 128 heads 40 -> 46
 // us, whose terms take the LDS of the second workgroup).
 //
-// 8192 tokens of 32 bfloat16 heads of 128 x 128: 118 us, of which local states 37 (168 MB), the states before each segment 12 (67 MB), outputs 69
-// (301 MB): each pass near the rate of a large copy (5.1 TB/s), reading K and V twice is what the split over the device costs.  Five
+// 8192 tokens of 32 bfloat16 heads of 128 x 128: 130 us, of which local states 37 (168 MB), the states before each segment 12 (67 MB), outputs 80
+// (301 MB; with one-term operands 69): the first two near the rate of a large copy (5.1 TB/s); reading K and V twice is what the split over the device costs.  Five
 // ragged f32 sequences (1683 tokens, 16 heads of 64 x 128): 40 us, bound by the f32 matrix instruction and three launches.
 constexpr int CH = 64;
 
@@ -212,7 +213,7 @@ template <typename T> struct Op;
 template <> struct Op<__bf16> {
     typedef mk_b8 F;
     // values a row of K and V (read down the columns: eight rows of 4 + 4 words side by side) and of Q (read along the rows) is padded by
-    static constexpr int PAD = 16, QPAD = 8, TERMS = 3;
+    static constexpr int PAD = 16, QPAD = 8, TERMS = 3, OUT_TERMS = 2;
     static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ bool finite(const mk_v4u &r) {  // of a 16-byte piece of a row
         bool ok = true;
@@ -223,7 +224,7 @@ template <> struct Op<__bf16> {
 };
 template <> struct Op<float> {
     typedef mk_f8v F;
-    static constexpr int PAD = 4, QPAD = 4, TERMS = 1;
+    static constexpr int PAD = 4, QPAD = 4, TERMS = 1, OUT_TERMS = 1;
     static __device__ __forceinline__ mk_f4 mma(F a, F b, mk_f4 c) {
 #pragma unroll
         for (int i = 0; i < 8; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -236,12 +237,18 @@ template <> struct Op<float> {
         return ok;
     }
 };
-// two result tiles (or any 8 values) as an operand
-template <typename T> __device__ __forceinline__ typename Op<T>::F operand(const mk_f4 &lo, const mk_f4 &hi) {
-    typename Op<T>::F f;
+// two result tiles (or any 8 values) as an operand, the sum of N terms, largest first
+template <typename T, int N> __device__ __forceinline__ void operand(const mk_f4 &lo, const mk_f4 &hi, typename Op<T>::F (&f)[N]) {
+    float r[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = (T)lo[i], f[4 + i] = (T)hi[i];
-    return f;
+    for (int i = 0; i < 4; i++) r[i] = lo[i], r[4 + i] = hi[i];
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            f[k][i] = (T)r[i];
+            if (k + 1 < N) r[i] -= (float)f[k][i];
+        }
 }
 // values 8 consecutive of a row
 __device__ __forceinline__ mk_b8 row8(const __bf16 *p) { return *(const mk_b8 *)p; }
@@ -327,11 +334,11 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
     typedef typename Op<T>::F F;
     constexpr bool OUT = MODE != LOCAL;
     // the state that only leads to the next outputs takes two terms (2^-17 beside its own rounding to bfloat16)
-    constexpr int TERMS = MODE == OUTPUT && Op<T>::TERMS > 2 ? 2 : Op<T>::TERMS;
+    constexpr int TERMS = MODE == OUTPUT && Op<T>::TERMS > 2 ? 2 : Op<T>::TERMS, OT = Op<T>::OUT_TERMS;
     constexpr int NT = tiles<T, DK, DV, MODE>(), NW = DV / 16 / NT, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
     __shared__ __attribute__((aligned(16))) T k_l[CH * LK], v_l[CH * LV], q_l[OUT ? CH * LQ : 8];
-    __shared__ F p_l[OUT ? 6 : 1][64];                  // scores: query tiles 0 .. 3 with keys 0 .. 31, query tiles 2, 3 with keys 32 .. 63
+    __shared__ F p_l[OT][OUT ? 6 : 1][64];              // scores: query tiles 0 .. 3 with keys 0 .. 31, query tiles 2, 3 with keys 32 .. 63
     __shared__ double b_l[2][CH];                       // sums of the log2 decays of a block and of the next
     __shared__ float w_l[2][CH], e_l[2][CH], last_l[2];  // 2^(b_m - b_i), scale * 2^(b_i), 2^(b_m)
     __shared__ int bad_l;
@@ -458,7 +465,10 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
                         }
                     }
                 }
-                p_l[f][lane] = operand<T>(pt[0], pt[1]);
+                F pf[OT];
+                operand<T>(pt[0], pt[1], pf);
+#pragma unroll
+                for (int k = 0; k < OT; k++) p_l[k][f][lane] = pf[k];
             }
         }
         // (a wave with few or no scores forms the next block's sums)
@@ -472,20 +482,21 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
             for (int ks = 0; ks < 2; ks++) vt[t][ks] = column8<LV>(v_l, ks, 16 * (NT * wave + t), g, n);
         if constexpr (OUT) {
             const bool plain = bad_l == c + 1;  // a value that is not finite: 0 times it must not reach earlier tokens
-            F sf[NT][KS];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int s = 0; s < KS; s++) sf[t][s] = operand<T>(S[2 * s][t], S[2 * s + 1][t]);
             mk_f4 o[NT][4];
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
+                F sf[NT][OT], qb[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const F qb = row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]);
+                for (int t = 0; t < NT; t++) operand<T>(S[2 * s][t], S[2 * s + 1][t], sf[t]);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) o[t][j] = Op<T>::mma(sf[t][s], qb, s ? o[t][j] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
-                }
+                for (int j = 0; j < 4; j++) qb[j] = row8(&q_l[(16 * j + n) * LQ + 32 * s + 8 * g]);
+#pragma unroll
+                for (int k = 0; k < OT; k++)  // several sums in turn
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int t = 0; t < NT; t++) o[t][j] = Op<T>::mma(sf[t][k], qb[j], s || k ? o[t][j] : mk_f4{0.0f, 0.0f, 0.0f, 0.0f});
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float e = e_l[u][16 * j + n];
@@ -496,17 +507,21 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
             }
             if (!plain) {
 #pragma unroll
-                for (int f = 0; f < 6; f++) {
-                    const F pb = p_l[f][lane];
+                for (int k = 0; k < OT; k++)
 #pragma unroll
-                    for (int t = 0; t < NT; t++) o[t][f < 4 ? f : f - 2] = Op<T>::mma(vt[t][f < 4 ? 0 : 1], pb, o[t][f < 4 ? f : f - 2]);
-                }
+                    for (int f = 0; f < 6; f++) {
+                        const F pb = p_l[k][f][lane];
+#pragma unroll
+                        for (int t = 0; t < NT; t++) o[t][f < 4 ? f : f - 2] = Op<T>::mma(vt[t][f < 4 ? 0 : 1], pb, o[t][f < 4 ? f : f - 2]);
+                    }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     for (int key = 0; key <= 16 * j + n; key++) {
                         const int r = key & 31;
-                        const float p = (float)p_l[key < 32 ? j : 2 + j][16 * ((r & 15) >> 2) + n][4 * (r >> 4) + (r & 3)];
+                        float p = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < OT; k++) p += (float)p_l[k][key < 32 ? j : 2 + j][16 * ((r & 15) >> 2) + n][4 * (r >> 4) + (r & 3)];
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll

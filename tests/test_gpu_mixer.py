@@ -650,3 +650,23 @@ def test_kv4_a_bfloat16_result_is_rounded_once(lens, news, nh, nkv, dk, rope):
             want, bound, mag = ref.attn(q[t], kk, vv, lens[b] - news[b] + i, scale)
             rounded_once(got[t], want, bound * U32 + U16 ** 2 * mag, f"sequence {b} row {i}")
             t += 1
+
+
+@pytest.mark.parametrize("nh,nkh,dk,dv", [(2, 2, 128, 128), (4, 2, 64, 128), (3, 1, 128, 64), (2, 2, 64, 64), (2, 1, 40, 72)])
+@pytest.mark.parametrize("lens,with_state", [([70, 0, 1, 64, 129], True), ([1000], True), ([100], False), ([900, 3, 300], True)])
+def test_linear_a_bfloat16_result_is_rounded_once(lens, with_state, nh, nkh, dk, dv):
+    """One workgroup a sequence, and segments.  The state and the weighted scores may enter their products, and where a state only leads to
+    later outputs its updates too, as two bfloat16 terms: twice U16^2."""
+    from microkimi_amd import mixer
+    rng = np.random.default_rng(41 + sum(lens) + dk)
+    B, T = len(lens), sum(lens)
+    q, k, v = rows(rng, (T, nkh, dk), "bf16"), rows(rng, (T, nkh, dk), "bf16"), rows(rng, (T, nh, dv), "bf16")
+    g = -(0.2 * rng.random((T, nh))).astype(np.float32)
+    state = rng.standard_normal((B, nh, dk, dv)).astype(np.float32) if with_state else np.zeros((B, nh, dk, dv), np.float32)
+    scale = dk ** -0.5
+    got, _ = mixer.linear_attn(*(to_dev(x, "bf16") for x in (q, k, v)), to_dev(g), to_dev(state) if with_state else None, scale, cu=cu_of(lens))
+    got, t = host(got), 0
+    for b, n in enumerate(lens):
+        want, _, mag, _ = ref.linear(q[t:t + n], k[t:t + n], v[t:t + n], g[t:t + n], state[b], scale)
+        rounded_once(got[t:t + n], want, ((2 * n + dk + 24) * U32 + 2 * U16 ** 2) * mag, f"sequence {b}")
+        t += n
