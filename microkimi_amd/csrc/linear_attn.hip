@@ -294,7 +294,8 @@ template <int LD> __device__ __forceinline__ mk_f8v column8(const float *tile, i
 template <int N> struct Int { static constexpr int value = N; };
 
 // A sequence is cut into segments of `per` blocks, each a slot of the workspace and a workgroup per head; sequence b has the slots from
-// at(b) / (64 per) + b on: never fewer than its segments (some stay empty), T / (64 per) + B in all, whatever the lengths are.
+// at(b) / (64 per) + b on: never fewer than its segments (some stay empty, those before the first sequence's too), T / (64 per) + B in all,
+// whatever the lengths are.
 struct LinSeg {
     int per;        // 0: a sequence is one workgroup per head, without a workspace
     mk_f4 *local;   // [slot][h][DK / 16][4 DV]: local states, then the states before each segment
@@ -354,7 +355,9 @@ __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL 
             else hi = mid;
         }
         b = lo;
-        c0 = max(slot - sg.first(a, b), 0) * sg.per;
+        c0 = slot - sg.first(a, b);
+        if (c0 < 0) return;  // a slot of the rows before the first sequence
+        c0 *= sg.per;
     }
     const int t0 = a.at(b), len = max(a.at(b + 1) - t0, 0), nch = (len + CH - 1) / CH, c1 = MODE == BOTH ? nch : min(c0 + sg.per, nch);
     if (MODE != BOTH && c0 >= c1) return;

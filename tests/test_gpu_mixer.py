@@ -670,3 +670,35 @@ def test_linear_a_bfloat16_result_is_rounded_once(lens, with_state, nh, nkh, dk,
         want, _, mag, _ = ref.linear(q[t:t + n], k[t:t + n], v[t:t + n], g[t:t + n], state[b], scale)
         rounded_once(got[t:t + n], want, ((2 * n + dk + 24) * U32 + 2 * U16 ** 2) * mag, f"sequence {b}")
         t += n
+
+
+# ------------------------------------------------------------------------------------------- rows before the first sequence
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkh,dk,dv", [(2, 1, 64, 64), (2, 2, 128, 128), (4, 2, 64, 128)])
+@pytest.mark.parametrize("cu,T", [([200, 1000], 1000), ([300, 700, 1500], 1600), ([513, 513, 1900, 1901], 1901), ([-7, 90, 5000], 1200)])
+def test_linear_rows_before_the_first_sequence_belong_to_nobody(cu, T, nh, nkh, dk, dv, dtype):
+    """Long enough for segments: every segment is computed once, from the state before it.  Entries outside 0 .. T count as the nearer bound."""
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    rng = np.random.default_rng(51 + T)
+    B, at = len(cu) - 1, np.clip(cu, 0, T)
+    q, k, v = rows(rng, (T, nkh, dk), dtype), rows(rng, (T, nkh, dk), dtype), rows(rng, (T, nh, dv), dtype)
+    g = -(0.1 * rng.random((T, nh))).astype(np.float32)
+    for a in (q, k, v, g):
+        a[:at[0]], a[at[-1]:] = np.nan, np.nan
+    state = rng.standard_normal((B, nh, dk, dv)).astype(np.float32)
+    out = torch.full((T, nh, dv), 7.0, dtype=to_dev(v[:1], dtype).dtype, device="cuda")
+    scale = dk ** -0.5
+    got, new = mixer.linear_attn(*(to_dev(x, dtype) for x in (q, k, v)), to_dev(g), to_dev(state), scale, cu=ints(cu), out=out)
+    got, new = host(got), host(new)
+    assert (got[:at[0]] == 7.0).all() and (got[at[-1]:] == 7.0).all()
+    for b in range(B):
+        s = slice(at[b], at[b + 1])
+        want, S, mag, M = ref.linear(q[s], k[s], v[s], g[s], state[b], scale)
+        f32 = (2 * len(want) + dk + 24) * U32      # (as in check_linear; bfloat16: two-term operands, twice U16^2)
+        if dtype == "bf16":
+            rounded_once(got[s], want, (f32 + 2 * U16 ** 2) * mag, f"sequence {b}")
+        else:
+            within(got[s], want, f32 * mag + 1e-30, f"sequence {b}")
+        within(new[b], S, f32 * M + 1e-30, f"state of sequence {b}")
