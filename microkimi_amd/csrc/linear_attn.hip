@@ -660,14 +660,17 @@ size_t segment_bytes(size_t n, size_t dk, size_t dv) { return n * dk * dv * 4 + 
 // A sequence needs four blocks on average, six of 128 bfloat16 columns, which two workgroups share when they are few (32 heads of 128 x 128
 // without / with: 256 tokens 20 / 24 us, 400 tokens 32 / 29 us; in f32 256 tokens 42 / 45 us, 320 tokens 53 / 47 us).
 // f32 heads wider than 64 x 64 leave room for one workgroup a compute unit: longer segments of equal sequences, so that all of them run at
-// once (2048 tokens of 32 heads of 128 x 128: 91 us, in segments of two blocks 100; 3241 of 24 heads 123 and 132 us).
+// once (2048 tokens of 32 heads of 128 x 128: 91 us, in segments of two blocks 100; 3241 of 24 heads 123 and 132 us).  From 129 heads on that
+// would be one segment a sequence, which is the work of the segments without their workgroups: none then (160 heads of 400 tokens without / one
+// segment 99 / 140 us, of 4096 tokens 859 / 1167 us; 5 sequences of 32 heads of 1024 tokens 220 / 360 us).
 int segment_blocks(size_t T, size_t B, size_t nh, size_t dk, size_t dv, bool bf16, bool ragged) {
     const size_t blocks = (T + CH - 1) / CH;
     if (B * nh > (ragged ? 256 : 191) || blocks < (bf16 && dv == 128 ? 6 : 4) * B) return 0;
     size_t per = least_segment(T, nh);
     if (!ragged && !bf16 && dk + dv > 128) {
-        const size_t most = 256 / (B * nh), even = ((T / B + CH - 1) / CH + most - 1) / most;
+        const size_t each = (T / B + CH - 1) / CH, most = 256 / (B * nh), even = (each + most - 1) / most;
         per = even > per ? even : per;
+        if (per >= each) return 0;
     }
     return (int)per;
 }

@@ -702,3 +702,27 @@ def test_linear_rows_before_the_first_sequence_belong_to_nobody(cu, T, nh, nkh, 
         else:
             within(got[s], want, f32 * mag + 1e-30, f"sequence {b}")
         within(new[b], S, f32 * M + 1e-30, f"state of sequence {b}")
+
+
+@pytest.mark.parametrize("T,B,nh,dk,dv", [(512, 1, 160, 64, 128), (1280, 2, 65, 128, 128), (300, 1, 191, 128, 64)])
+def test_linear_equal_f32_sequences_are_not_cut_into_one_segment_each(T, B, nh, dk, dv):
+    """A segment a sequence is the same workgroups three times over: such calls leave their workspace alone."""
+    from microkimi_amd._lib import F32, check, lib
+    torch = torch_cuda()
+    rng = np.random.default_rng(61)
+    q, k, v = (rng.standard_normal((T, h, w)).astype(np.float32) for h, w in ((1, dk), (1, dk), (nh, dv)))
+    g = -(0.1 * rng.random((T, nh))).astype(np.float32)
+    tq, tk, tv, tg = to_dev(q), to_dev(k), to_dev(v), to_dev(g)
+    n = lib.mk_linear_attn_workspace_bytes(T, B, nh, dk, dv)
+    ws = torch.full((n,), 77, dtype=torch.uint8, device="cuda")
+    out, S = torch.empty((T, nh, dv), device="cuda"), torch.empty((B, nh, dk, dv), device="cuda")
+    check(lib.mk_dev_linear_attn(F32, tq.data_ptr(), dk, tk.data_ptr(), dk, tv.data_ptr(), nh * dv, tg.data_ptr(), nh, T, None, B, nh, 1, dk, dv, 0.1, None,
+                                 S.data_ptr(), ws.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert (ws == 77).all()
+    out, S, m = host(out), host(S), T // B
+    for b in range(B):
+        s, h = slice(b * m, (b + 1) * m), [0, 1, nh // 2, nh - 1]
+        want, W, mag, M = ref.linear(np.repeat(q[s], 4, 1), np.repeat(k[s], 4, 1), v[s][:, h], g[s][:, h], np.zeros((4, dk, dv), np.float32), 0.1)
+        f32 = (2 * m + dk + 24) * U32
+        within(out[s][:, h], want, f32 * mag + 1e-30, f"sequence {b}")
+        within(S[b][h], W, f32 * M + 1e-30, f"state of sequence {b}")
