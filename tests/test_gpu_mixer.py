@@ -726,3 +726,19 @@ def test_linear_equal_f32_sequences_are_not_cut_into_one_segment_each(T, B, nh, 
         f32 = (2 * m + dk + 24) * U32
         within(out[s][:, h], want, f32 * mag + 1e-30, f"sequence {b}")
         within(S[b][h], W, f32 * M + 1e-30, f"state of sequence {b}")
+
+
+def test_calls_by_torchs_public_stream_and_device(monkeypatch):
+    """What mixer uses where torch has no internal forms of them, under a stream of its own."""
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    x = to_dev(rows(np.random.default_rng(71), (3, 2, 64), "f32"))
+    want, _ = mixer.qk_norm_rope(x, None)
+    torch.cuda.synchronize()
+    with monkeypatch.context() as m:
+        m.setattr(mixer, "_current_device", torch.cuda.current_device)
+        m.setattr(mixer, "_raw_stream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got, _ = mixer.qk_norm_rope(x, None)
+        torch.cuda.synchronize()
+    assert torch.equal(got, want)

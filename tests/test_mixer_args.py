@@ -145,3 +145,20 @@ def test_the_cache_struct_is_the_same_in_the_header_the_binding_and_the_shim():
     kinds = {"size_t": "usize", "uint8_t": "u8", "uint16_t": "u16", "int32_t": "i32"}
     assert rust == [(n, p, kinds[k]) for n, p, k in header]
     assert [(n, t is C.c_size_t) for n, t in Kv4Cache._fields_] == [(n, not p) for n, p, _ in header]
+
+
+def test_the_package_imports_where_torch_lacks_its_internal_names():
+    """The host entry points need neither a stream nor a device."""
+    import os
+    import pathlib
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "import microkimi_amd\n"
+            "print(microkimi_amd._lib.lib.mk_enabled_now(), callable(microkimi_amd.mixer.qk_norm_rope))\n")
+    root = str(pathlib.Path(__file__).resolve().parents[1])
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, env=dict(os.environ, PYTHONPATH=root), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert run.returncode == 0, run.stdout
+    assert run.stdout.split()[-2:] == ["1", "True"]
