@@ -710,7 +710,7 @@ int check_linear(int dtype, const void *q, size_t qs, const void *k, size_t ks, 
     MK_REQUIRE(B >= 1 && B <= 65535 && T <= 0x3FFFFFFF, "bad token or sequence count");
     MK_REQUIRE(nh >= 1 && nh <= 65535 && nkh >= 1 && nh % nkh == 0, "the value heads must be a multiple of the key heads");
     MK_REQUIRE(dk >= 8 && dk <= 256 && dk % 8 == 0 && dv >= 8 && dv <= 256 && dv % 8 == 0, "head widths must be multiples of 8 up to 256");
-    MK_REQUIRE(g && state_out && (T == 0 || (q && k && v && out)), "null pointer");
+    MK_REQUIRE(state_out && (T == 0 || (q && k && v && g && out)), "null pointer");
     MK_REQUIRE(qs % 8 == 0 && ks % 8 == 0 && vs % 8 == 0, "token strides must be multiples of 8 values");
     MK_REQUIRE(qs <= 0x7FFFFF && ks <= 0x7FFFFF && vs <= 0x7FFFFF, "a token stride is out of range");
     MK_REQUIRE(T <= 1 || (qs >= nkh * dk && ks >= nkh * dk && vs >= nh * dv && (gs == 0 || gs >= nh)), "a token stride is shorter than a token's heads");

@@ -318,6 +318,8 @@ def linear_attn_step(q, k, v, g, state=None, scale=1.0, out=None, state_out=None
     """linear_attn for one token of each of B sequences (mk_dev_linear_attn_step): q, k [B, nkh, dk], v [B, nh, dv], g [B, nh] or
     [nh], state [B, nh, dk, dv].  Returns (out [B, nh, dv], state_out)."""
     dt, q, qs, k, ks, v, vs, g, gs, B, nh, nkh, dk, dv, state, state_out, out = _linear_args(q, k, v, g, state, q.shape[0], out, state_out)
+    if B == 0:
+        return out, state_out
     check(lib.mk_dev_linear_attn_step(dt, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), gs, B, nh, nkh, dk, dv, scale,
                                       None if state is None else state.data_ptr(), state_out.data_ptr(), out.data_ptr(), _start(q)))
     return out, state_out

@@ -742,3 +742,25 @@ def test_calls_by_torchs_public_stream_and_device(monkeypatch):
             got, _ = mixer.qk_norm_rope(x, None)
         torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk,dv", [(64, 128), (40, 72)])
+@pytest.mark.parametrize("per_token", [True, False])
+def test_linear_calls_without_a_token(dk, dv, per_token, dtype):
+    """No tokens: nothing comes out and every state stays as it is; no sequences of one token: nothing at all."""
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    q, v = to_dev(np.zeros((0, 2, dk)), dtype), to_dev(np.zeros((0, 4, dv)), dtype)
+    g = torch.zeros((0, 4) if per_token else 4, device="cuda")
+    S = to_dev(np.random.default_rng(81).standard_normal((3, 4, dk, dv)))
+    for cu in (None, ints([0, 0, 0, 0])):
+        out, new = mixer.linear_attn(q, q, v, g, S, cu=cu)
+        assert out.shape == (0, 4, dv) and torch.equal(new, S)
+        out, new = mixer.linear_attn(q, q, v, g, B=2)
+        assert out.shape == (0, 4, dv) and new.shape == (2, 4, dk, dv) and not new.any()
+    out, new = mixer.linear_attn_step(q, q, v, g)
+    assert out.shape == (0, 4, dv) and out.dtype == v.dtype and new.shape == (0, 4, dk, dv)
+    mine = torch.empty((0, 4, dv), dtype=v.dtype, device="cuda")
+    out, new = mixer.linear_attn_step(q, q, v, g, S[:0], out=mine)
+    assert out is mine and new.shape == (0, 4, dk, dv)
