@@ -424,7 +424,8 @@ int mk_dev_mla_heads_q8_attn(const int8_t *kq, const float *ks, const float *kr,
  * A batch of sequences: the rows of a call lie one behind the other, cu [B + 1] int32 (device) says where each sequence's
  * begin and the last one's end; cu NULL: T / B rows each (T % B == 0).  Entries of cu outside 0 .. T are taken as the nearer
  * bound; rows that belong to no sequence are neither read nor written.  A token's heads are contiguous, tokens may be
- * further apart (a row stride in values, a multiple of 8: q, k, v may be slices of one projection's rows).
+ * further apart (a row stride in values, a multiple of 8: q, k, v may be slices of one projection's rows).  Outputs must not
+ * overlap inputs, except where a call says so.
  *
  * mk_dev_qk_norm_rope: RMS norm of every query head [T][nh][hd] and key head [T][nkv][hd] with the rotation of the token's
  * position, one pass:

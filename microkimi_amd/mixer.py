@@ -4,8 +4,9 @@ cache held in 4 bits (several sequences, grouped-query heads), and linear attent
 Rows are f32 or bfloat16 tensors on the current device, [tokens, heads, width]; a token's heads must lie one behind the other, the
 tokens may be further apart (slices of one projection's rows are taken as they are, other layouts are copied).  A batch of
 sequences: rows one sequence behind the other, cu [B + 1] int32 on the device = where each one's rows begin (None: equally many
-rows each).  Every call only enqueues work on the current stream and takes what it needs from torch's allocator, so calls may
-be captured into graphs and run on several streams."""
+rows each).  Outputs that the caller gives must not overlap the inputs, except where a call says that it works in place.  Every call
+only enqueues work on the current stream and takes what it needs from torch's allocator, so calls may be captured into graphs and run
+on several streams."""
 import ctypes as C
 
 import torch
@@ -89,6 +90,14 @@ def _result(out, ref, shape, name, dtype=None):
     return out
 
 
+def _apart(out, name, *inputs):
+    """Refuses an output of the caller's that begins where an input begins which other workgroups may still read."""
+    at = out.data_ptr()
+    for t in inputs:
+        if t is not None and t.data_ptr() == at and at:
+            raise ValueError(f"{name} must not overlap the call's inputs")
+
+
 def _workspace(ref, n):
     """(n bytes of device memory for a call, their address), or none."""
     if n == 0:
@@ -142,6 +151,10 @@ def qk_norm_rope(q, k, cos=None, sin=None, pos=None, wq=None, wk=None, eps=1e-6,
         _same(ref, pos, "pos", torch.int32)
         if pos.dim() != 1 or pos.shape[0] != T or not pos.is_contiguous():
             raise ValueError(f"pos must be {T} contiguous values")
+    if q_out is not None:
+        _apart(q_out, "q_out", k)
+    if k_out is not None:
+        _apart(k_out, "k_out", q, q_out)
     qr, qp, qs, nh, wq, wqp, qo, qop = _heads(ref, q, wq, q_out, T, hd, "q")
     kr, kp, ks, nkv, wk, wkp, ko, kop = _heads(ref, k, wk, k_out, T, hd, "k")
     check(lib.mk_dev_qk_norm_rope(dt, qp, qs, nh, kp, ks, nkv, T, hd, 1 if norm else 0, wqp, wkp, eps, _ptr(cos), _ptr(sin), n_pos, _ptr(pos), rot,
@@ -289,6 +302,10 @@ def _linear_args(q, k, v, g, state, B, out, state_out):
             g = g.contiguous()
         gs = g.stride(0) if T > 1 else nh
     shape = (B, nh, dk, dv)
+    if state_out is not None:
+        _apart(state_out, "state_out", q, k, v)
+    if out is not None:
+        _apart(out, "out", q, k, state, state_out)
     if state is not None:
         state = _f32(q, state, "state", shape)
     state_out = _result(state_out, q, shape, "state_out", torch.float32)

@@ -802,3 +802,31 @@ def test_linear_values_that_are_not_finite_in_long_prompts(at, dk, dv, dtype):
         rest = torch.arange(T, device="cuda") != at
         assert torch.equal(got[rest], want[rest]) and torch.equal(got[:, 1], want[:, 1]) and torch.equal(S, W)
         assert not torch.isfinite(got[at, 0]).any()
+
+
+def test_outputs_that_overlap_what_a_call_still_reads_are_refused():
+    """Two workgroups that share a head's columns read all of its query: a result in the same place would overwrite it under the other."""
+    from microkimi_amd import mixer
+    torch = torch_cuda()
+    T, h, d = 3, 2, 128
+    q, k, v = (torch.zeros((T, h, d), device="cuda") for _ in range(3))
+    g, pool = torch.zeros(h, device="cuda"), torch.zeros((T + 1, h, d, d), device="cuda")
+    for call, S, S1 in ((mixer.linear_attn, pool[:1], pool[1:2]), (mixer.linear_attn_step, pool[:T], None)):
+        for x in (q, k):
+            with pytest.raises(ValueError, match="overlap"):
+                call(q, k, v, g, S, out=x)
+        if S1 is not None:
+            out, new = call(q, k, v, g, S, out=torch.empty_like(v), state_out=S1)     # side by side is not an overlap
+            assert new is S1
+        out, new = call(q, k, v, g, S, state_out=S)
+        assert new is S
+    row = torch.zeros((1, 4 * h, d), device="cuda")                                     # one token: slices of one row
+    out, _ = mixer.linear_attn_step(row[:, :h], row[:, h:2 * h], row[:, 2 * h:3 * h], g, out=row[:, 3 * h:])
+    assert out.data_ptr() == row[:, 3 * h:].data_ptr()
+    fused = torch.zeros((T, 3 * h, d), device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        mixer.linear_attn(fused[:, :h], fused[:, h:2 * h], fused[:, 2 * h:], g, out=fused.view(-1)[:T * h * d].view(T, h, d))
+    with pytest.raises(ValueError, match="overlap"):
+        mixer.qk_norm_rope(q, k, q_out=k)
+    with pytest.raises(ValueError, match="overlap"):
+        mixer.qk_norm_rope(q, k, k_out=q)
