@@ -422,7 +422,7 @@ int mk_dev_mla_heads_q8_attn(const int8_t *kq, const float *ks, const float *kr,
  * matrix cores - softmax weights, weighted scores, a state - enters as two bfloat16 terms, 17 bits, or three).
  *
  * A batch of sequences: the rows of a call lie one behind the other, cu [B + 1] int32 (device) says where each sequence's
- * begin and the last one's end; cu NULL: T / B rows each (T % B == 0).  Entries of cu outside 0 .. T are taken as the nearer
+ * begin and the last one's end, never decreasing; cu NULL: T / B rows each (T % B == 0).  Entries of cu outside 0 .. T are taken as the nearer
  * bound; rows that belong to no sequence are neither read nor written.  A token's heads are contiguous, tokens may be
  * further apart (a row stride in values, a multiple of 8: q, k, v may be slices of one projection's rows).  Outputs must not
  * overlap inputs, except where a call says so.
@@ -469,7 +469,8 @@ int mk_dev_kv4_to_f32(const mk_kv4_cache *c, size_t n, float *k, float *v, void 
  * 0 ..= lens - m + i (m = 1: a decode step; more: a prompt, causal).  q [T][nh][dk + rope], out [T][nh][dv] contiguous; query
  * head h reads kv head h / (nh / nkv).  s_j = scale * q . k_j, out = sum softmax(s)_j v_j.  A row that has no position to
  * attend (an empty sequence) gives zeros, one that would have to attend a position beyond cap gives NaN.
- * max_len: an upper bound of lens, if the caller has one (0: none); it only steers how the work is split.
+ * max_len: an upper bound of lens, if the caller has one (0: none); it only steers how the work is split, which is by the capacity
+ * without it: worth giving where cap is many times what is held.
  * workspace: mk_kv4_attn_workspace_bytes(c, T, nh) bytes, 256-byte aligned (0: may be NULL), one for each call that may run at
  * the same time. */
 size_t mk_kv4_attn_workspace_bytes(const mk_kv4_cache *c, size_t T, size_t nh);
@@ -481,7 +482,8 @@ int mk_dev_kv4_attn(const mk_kv4_cache *c, int dtype, const void *q, size_t q_st
  * q, k [T][nkh][dk], v [T][nh][dv], out [T][nh][dv] contiguous (value head h reads key head h / (nh / nkh)); g: log decays f32,
  * [T] rows of nh at g_stride, or, g_stride == 0, one constant per head [nh]; -inf empties the state.  state [B][nh][dk][dv]
  * (NULL: zeros) is the state before the call, state_out the one after it; they may be the same memory.  A sequence without
- * tokens keeps its state.  dk, dv multiples of 8 up to 256; pointers 16-byte aligned.
+ * tokens keeps its state (g, q, k, v and out may be NULL when T == 0).  dk, dv multiples of 8 up to 256, strides up to 8388607; pointers
+ * 16-byte aligned.
  * _attn is the form for prompts (workspace: mk_linear_attn_workspace_bytes, 256-byte aligned, 0: may be NULL, one for each call that may
  * run at the same time), _step the one for a single token of each of B sequences (rows b of q, k, v, g and out). */
 size_t mk_linear_attn_workspace_bytes(size_t T, size_t B, size_t nh, size_t dk, size_t dv);

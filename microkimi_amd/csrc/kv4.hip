@@ -1,9 +1,8 @@
-// Attention over a KV cache held in 4 bits (MXFP4: e2m1 nibbles, an e8m0 byte per 32 values), for a batch of sequences.
+// A KV cache held in 4 bits (MXFP4: e2m1 nibbles, an e8m0 byte per 32 values), for a batch of sequences (attention: kv4_attn.hip).
 //
 //   append   rows of every sequence behind the positions it holds; K and V per kv head as MXFP4, an optional K tail of `rope`
 //            values shared by the heads (taken from head 0) as bfloat16
 //   to_f32   the values the cache stands for
-//   attn     s_j = scale * (q . k_j), softmax over the positions a row may see, o = sum p_j v_j; query heads nh / nkv to a kv head
 //
 // Quantization of a block: e = the smallest exponent with 6 * 2^e >= max|x|, clamped to [-127, 125]; the nearest level, upwards at
 // a midpoint (the rule of the MXFP4 codec); NaN becomes 0 and what lies beyond 6 * 2^125 saturates, so that the cache holds
@@ -18,6 +17,7 @@ namespace {
 __device__ __forceinline__ int advanced(int held, int n) { return (int)min((int64_t)held + max(n, 0), (int64_t)1 << 30); }
 
 // Two rows a wave: 6340 rows of 2048 values 12.3 us (four rows the same, one row 14.8), 16 rows of one token 5.0 us (four rows 6.8, one 3.8).
+// A push of 16 tokens with the launch that advances lens: 5.3 us in a graph.
 constexpr int APPEND_ROWS = 2;
 
 // One wave: 64 items of ROWS rows of the call.  An item is 8 values: nkv * dk / 8 of K, nkv * dv / 8 of V, rope / 8 of the K tail.
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256) void kv4_advance_kernel(MkKv4 c, MkSeqs s, int
 
 // A thread: 4 values (an item of a position's K or V rows) of SNAP positions of a sequence, so that a wave stores 1 KiB in a row; positions
 // a sequence does not hold are zero.  HBM-bound: 1500 positions of 96 heads of 192 + 128 (184 MB written) 32 us, 5.8 TB/s (with two and
-// four items a thread 34.5 and 37.4 us); four sequences of 2048 positions of 8 heads of 128 + 128 12.4 us.
+// four items a thread 34.5 and 37.4 us); four sequences of 2048 positions of 8 heads of 128 + 128 13.0 us.
 constexpr int SNAP = 4;
 
 __global__ __launch_bounds__(256) void kv4_to_f32_kernel(MkKv4 c, int n, int parts, float *__restrict__ k, float *__restrict__ v) {

@@ -33,7 +33,8 @@ constexpr int GT = 256;  // positions of a tile: one a thread
 
 // One workgroup: (row, query head, split).  Scores: a thread takes a position of the tile.  Output: a thread takes 8 values (one
 // dword) of V for every (256 / (dv / 8))-th position of the tile.  Every cache byte is read once per query head, so this is the
-// form for widths that the matrix kernels below do not take.
+// form for widths that the matrix kernels below do not take (one token over 4096 positions, 16 heads to 2 kv heads, bfloat16: 42 us at 96 | 96, 63 at
+// 192 | 128, 203 at 512 + 64 | 512; 64 rows 0.87, 1.41 and 4.49 ms).
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_attn_any_kernel(MkKv4 c, MkSeqs s, AttnArgs a) {
     __shared__ float q_l[512 + 64], p_l[GT], red_l[8], acc_l[256 * 9];
@@ -495,8 +496,9 @@ __global__ __launch_bounds__(256, DK == 256 && sizeof(T) == 4 ? 1 : 2) void kv4_
 // ----------------------------------------------------------------------- many query columns: the workgroup shares K and V
 //
 // 512 rows behind 3584 positions, 96 heads of 128 + 64 | 128 in bfloat16 (121 GFLOP): 200 us, 605 TFLOP/s (a large library product:
-// 1085).  Operand reads from LDS (80 KB a step and workgroup) alone take 96 us, the matrix cores 69 (49 without the weights' second term).
-// 32 columns a wave would halve the reads, but 128 columns a workgroup leave 384 of them to 512 places.
+// 1085); 244 us in a row of calls without pauses, when the card lowers its clock.  Operand reads from LDS (80 KB a step and workgroup) alone take
+// 96 us, vector issue 95, the matrix cores 68 (49 without the weights' second term).  32 columns a wave would halve the reads, but 128 columns a
+// workgroup leave 384 of them to 512 places.
 //
 // One workgroup: (tile of 64 query columns, 16 a wave; kv head; chunk of the context), 32 positions a step.  Waves 0 and 1 turn the K
 // rows of 16 positions each into bfloat16 operands in LDS, waves 2 and 3 the V rows (as in the kernel above, so no transposed read
@@ -800,7 +802,9 @@ Form form_of(const mk_kv4_cache *c, size_t T, size_t group) {
     return T * group <= FEW * c->B && c->cap >= 32 ? FEW : MANY;
 }
 
-// Chunks that a context is cut into when `pairs` (column tile, kv head) walk `len` positions each.
+// Chunks that a context is cut into when `pairs` (column tile, kv head) walk `len` positions each.  `len` is max_len or the capacity, for the host does not
+// read lens: in a cache with much room the chunks are longer than what is held asks for (8 kv heads of 128 | 128, one row over 2048 positions:
+// capacity 2048 10.9, 16384 11.8, 131072 16.9 us; 64 rows over 4096: capacity 4096 39, 32768 73, 131072 100 us; with max_len as with the tight cache).
 //
 // Few columns: about 1024 chunks fill the 256 compute units; below 256 positions (two steps a wave) a chunk is start and end only,
 // above 1024 one long sequence among short ones is a tail (32 ragged sequences of up to 16384 positions: 30.2 / 24.2 / 27.0 us in chunks of

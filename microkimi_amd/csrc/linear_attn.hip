@@ -28,7 +28,8 @@ struct LinArgs {
 //
 // One workgroup: (64 columns of dv, value head, sequence).  Thread (rg, cg) = (tid / 16, tid % 16) holds rows rg + 16 i,
 // columns 4 cg .. 4 cg + 3 of the slice in registers: the state is read and written once, in runs of 256 bytes.  The tokens'
-// rows go through LDS, STAGE at a time.
+// rows go through LDS, STAGE at a time.  For widths that the blocks below do not take; bound by two barriers a token (1024 tokens of 16
+// bfloat16 heads of 96 x 96: 0.80 ms, of 256 x 256 1.24 ms).
 constexpr int COLS = 64, STAGE = 8;
 
 template <typename T> __device__ __forceinline__ float ldf(const T *p) { return (float)*p; }
@@ -203,9 +204,10 @@ int launch_token(const LinArgs &a, hipStream_t st) {
 // f32 rows: the same on the f32 matrix instruction (in three bfloat16 terms, six products: 128 x 128 heads 100 -> 95 us, but 64 x 128 heads 40 -> 46
 // us, whose terms take the LDS of the second workgroup).
 //
-// 8192 tokens of 32 bfloat16 heads of 128 x 128: 130 us, of which local states 37 (168 MB), the states before each segment 12 (67 MB), outputs 80
-// (301 MB; with one-term operands 69): the first two near the rate of a large copy (5.1 TB/s); reading K and V twice is what the split over the device costs.  Five
-// ragged f32 sequences (1683 tokens, 16 heads of 64 x 128): 40 us, bound by the f32 matrix instruction and three launches.
+// 8192 tokens of 32 bfloat16 heads of 128 x 128: 130 us, of which local states 38 (168 MB), the states before each segment 12 (67 MB), outputs 78
+// (301 MB, 22 % of the matrix cores' time; with one-term operands 69).  The first two move their bytes at the rate of a large copy (5.1 TB/s), the
+// outputs at 4.0; reading K and V twice is what the split over the device costs.  Five ragged f32 sequences (1683 tokens, 16 heads of
+// 64 x 128): 40 us, bound by the f32 matrix instruction and three launches.
 constexpr int CH = 64;
 
 typedef float mk_f8v __attribute__((ext_vector_type(8)));
@@ -334,7 +336,7 @@ template <typename T, int DK, int DV, Mode MODE>
 __global__ __launch_bounds__((DV * 4 / tiles<T, DK, DV, MODE>()), MODE == LOCAL ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 4 && DK > DV ? 1 : 2) void linear_block_kernel(LinArgs a, LinSeg sg) {
     typedef typename Op<T>::F F;
     constexpr bool OUT = MODE != LOCAL;
-    // the state that only leads to the next outputs takes two terms (2^-17 beside its own rounding to bfloat16)
+    // the state that only leads to the next outputs takes its updates as two terms, as it enters them (2^-16 of a value at most)
     constexpr int TERMS = MODE == OUTPUT && Op<T>::TERMS > 2 ? 2 : Op<T>::TERMS, OT = Op<T>::OUT_TERMS;
     constexpr int NT = tiles<T, DK, DV, MODE>(), NW = DV / 16 / NT, TH = 64 * NW, KT = DK / 16, KS = DK / 32, LK = DK + Op<T>::PAD, LV = DV + Op<T>::PAD, LQ = DK + Op<T>::QPAD;
     constexpr int E = 16 / sizeof(T), KP = CH * DK / E / TH, VP = CH * DV / E / TH;  // values of a 16-byte piece; pieces a thread moves
@@ -653,12 +655,12 @@ size_t segment_bytes(size_t n, size_t dk, size_t dv) { return n * dk * dv * 4 + 
 
 // Blocks of a segment, 0: no segments.  Without them a (sequence, head) is one workgroup; with them the keys and values are read twice
 // (local states first, then the outputs from the right states), and a long sequence beside short ones spreads over the device.
-// As many as two workgroups a compute unit ask for: 8192 tokens of 32 heads 118 us, as 768 or 1024 workgroups 132 and 136 us.
-// Equal lengths (no cu) are better off without from 192 heads on (bfloat16, 128 x 128; without / with): 192 heads of 400 tokens 43 / 64 us, of 1500
-// tokens 135 / 162 us; 128 heads of 400 tokens 41 / 48 us, of 1500 tokens 125 / 90 us.  What cu holds is not known here: up to 256 heads it
-// is taken for ragged (8 sequences of 24 heads, 1 .. 6000 tokens long: 340 / 125 us).
+// As many as two workgroups a compute unit ask for (8192 tokens of 32 heads, with one-term operands: 118 us, as 768 or 1024 workgroups 132 and
+// 136 us).  Equal lengths (no cu) are better off without from 192 heads on (bfloat16, 128 x 128; without / with): 192 heads of 1500 tokens 154 / 176 us,
+// 176 heads 150 / 164, 160 heads 145 / 124, 128 heads 106 / 98; of 400 tokens 52 / 67, 48 / 64, 48 / 62 and 37 / 51 us, for which the bound is high.
+// What cu holds is not known here: up to 256 heads it is taken for ragged (8 sequences of 24 heads, 1 .. 6000 tokens long: 340 us without, 137 with).
 // A sequence needs four blocks on average, six of 128 bfloat16 columns, which two workgroups share when they are few (32 heads of 128 x 128
-// without / with: 256 tokens 20 / 24 us, 400 tokens 32 / 29 us; in f32 256 tokens 42 / 45 us, 320 tokens 53 / 47 us).
+// without / with: 256 tokens 21 / 27 us, 400 tokens 33 / 31 us; in f32 256 tokens 44 / 46 us, 320 tokens 54 / 48 us).
 // f32 heads wider than 64 x 64 leave room for one workgroup a compute unit: longer segments of equal sequences, so that all of them run at
 // once (2048 tokens of 32 heads of 128 x 128: 91 us, in segments of two blocks 100; 3241 of 24 heads 123 and 132 us).  From 129 heads on that
 // would be one segment a sequence, which is the work of the segments without their workgroups: none then (160 heads of 400 tokens without / one
@@ -694,8 +696,8 @@ int launch_blocks(const LinArgs &a, const LinSeg &sg, hipStream_t st) {
 }
 template <typename T>
 int launch_blocks(LinArgs a, const LinSeg &sg, hipStream_t st) {
-    // While heads leave compute units free, two workgroups share a head of 128 columns (32 heads of 128 x 128, 70 tokens: f32 30 -> 23 us, bfloat16
-    // 13.3 -> 11.6 us; 128 heads of 100 tokens 15.4 -> 14.0 us; 192 f32 heads would take 33 for 20 us)
+    // While heads leave compute units free, two workgroups share a head of 128 columns (128 x 128, one workgroup / two: 32 heads of 70 tokens f32 30 / 23,
+    // bfloat16 15.6 / 12.1 us; 128 heads of 100 tokens 32 / 28 and 16.5 / 13.6 us; 192 heads 34 / 52 and 18 / 19 us)
     if (sg.per == 0 && a.dv == 128 && (size_t)a.B * a.nh <= SLICED) {
         a.slices = 2;
         return a.dk == 64 ? launch_blocks<T, 64, 64>(a, sg, st) : launch_blocks<T, 128, 64>(a, sg, st);

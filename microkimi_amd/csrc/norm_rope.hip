@@ -8,7 +8,7 @@
 // lanes, 8 values (one or two 16-byte loads) each: the sum of squares is log2(LPR) exchanges, a pair (i, i + rot / 2) one
 // exchange per value.  A group of LPR lanes keeps the token's table values and the weights in registers and walks its heads.
 // HBM-bound from some hundred tokens on (8192 tokens of 64 + 8 bfloat16 heads of 128: 62 us, 4.9 TB/s, a large copy 5.1); a
-// single token is the launch (3.3 us).
+// single token is the launch (3.7 us).
 #include "mk_mixer.h"
 
 namespace {
@@ -130,7 +130,7 @@ int launch(NormRopeArgs a, size_t n_tok, int halves, hipStream_t st) {
     constexpr int GROUPS = 256 / LPR;
     // From 1024 tokens on a token is one workgroup: its heads share the table's row and the weights, and the device is full (8192 tokens of
     // 64 + 8 bfloat16 heads of 128: 62 us, with one head a group of lanes 77 us).  Below, every group of lanes gets one head (777
-    // tokens of 96 + 96 f32 heads of 192: 52 us, as one workgroup a token 59 us).
+    // tokens of 96 + 96 f32 heads of 192: 52 us, as one workgroup a token 59 us).  Nothing between the two was measured.
     a.apart = n_tok < 1024;
     a.parts = a.apart ? ((a.nh > a.nkv ? a.nh : a.nkv) + GROUPS - 1) / GROUPS : 1;
     const size_t grid = n_tok * (size_t)a.parts * (a.apart ? 2 : 1);

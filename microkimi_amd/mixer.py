@@ -264,7 +264,7 @@ class KvCache4:
         """Softmax attention of the rows pushed last: q [T, nh, dk + rope], the m rows of a sequence are its last m positions, each
         attends what lies before it and itself (one row: a decode step; a prompt: causal).  nh a multiple of nkv.  Returns
         [T, nh, dv].  max_len: an upper bound of the sequences' lengths, if the caller keeps one (steers the split of the work
-        only)."""
+        only, which goes by the capacity without it: worth giving where that is many times what is held)."""
         dt = _code(q)
         _same(self.lens, q, "q", q.dtype)
         q, stride = _rows(q, "q", self.dk + self.rope)
